@@ -263,6 +263,81 @@ int ie_attention_decode(ie_dtype dt, int R, int rows_per_seq, int n_q_heads, int
                         int64_t cache_batch_stride, int cache_rows, const int* positions, int pos0,
                         void* out, int64_t ld_out, void* stream);
 
+/* ---- paged key/value cache ------------------------------------------------
+ * No counterpart in the reference (its cache is one contiguous block). One
+ * layer's cache is a pool of pages of page_size rows; sequence b's row j is
+ * row j % page_size of page page_table[b][j / page_size]. Strides are in
+ * elements, multiples of 8; rows of head_dim elements are contiguous, and the
+ * pool may be ordered [page][head][row] or [page][row][head], padded or not.
+ * k and v share the layout. head_dim 64 or 128; page_size a power of two from
+ * 16 to 256 (IE_ERR_UNSUPPORTED otherwise). */
+typedef struct ie_paged_cache {
+  void* k;
+  void* v;
+  int num_pages, page_size, n_kv_heads, head_dim;
+  int64_t page_stride, head_stride, row_stride;
+} ie_paged_cache;
+
+/* A call's new tokens are packed rows: sequence b owns rows q_start[b] ..
+ * q_start[b + 1] - 1 (device array [B + 1], not decreasing; a sequence may own
+ * none) and they sit at the last positions of its kv_len[b] cache rows (device
+ * array [B], new rows included). T is the number of rows the buffers hold:
+ * rows no sequence owns are not read and not written. page_table is a device
+ * array [B][max_pages] (row stride ld_table); entries for rows nobody asks for
+ * may hold anything. All three are read when the kernels run, so a captured
+ * graph follows them. What lies outside the call's extents (a page outside
+ * the pool, more rows than max_pages pages hold, more than max_q new tokens of
+ * one sequence, a row outside T) is not accessed: it sets IE_ERR_INVALID_ARG
+ * in ie_device_status, and the rows concerned are undefined. */
+
+/* Per-head RMSNorm and rotation of the new tokens' queries and keys, with
+ * keys and values written to their pages, in one pass: for each head row x of
+ * q and k, y = x * rsqrt(mean(x^2) + eps) * weight (weight [head_dim] in dt;
+ * NULL: no norm of that operand), then rotated by halves at the token's
+ * position p, as ie_qkv does: (y[d], y[d + D/2]) -> (y[d] c - y[d + D/2] s,
+ * y[d + D/2] c + y[d] s) with c, s = rope_cos/sin[p][d] ([rope_rows][D/2]
+ * fp32; NULL, NULL: no rotation). All fp32, rounded once. Rotated queries go
+ * to q_out (which may be q itself, with the same strides), keys and values to
+ * the cache; values are copied. Row t, head h of q lies at q + t * ldq + h *
+ * q_head_stride elements, and so for k, v and q_out: the three may be columns
+ * of one projection's output, or head-major. A token whose position has no
+ * cache row or no rotation row is skipped (IE_ERR_INVALID_ARG in
+ * ie_device_status). Two tokens must not share a cache row. */
+int ie_qk_norm_rope_paged(ie_dtype dt, int B, int T, int n_q_heads,
+                          const void* q, int64_t ldq, int64_t q_head_stride,
+                          const void* k, int64_t ldk, int64_t k_head_stride,
+                          const void* v, int64_t ldv, int64_t v_head_stride,
+                          const void* q_weight, const void* k_weight, float eps,
+                          const float* rope_cos, const float* rope_sin, int rope_rows,
+                          const ie_paged_cache* cache, const int* page_table, int64_t ld_table, int max_pages,
+                          const int* q_start, const int* kv_len,
+                          void* q_out, int64_t ldo, int64_t o_head_stride, void* stream);
+
+/* Causal grouped-query attention of the new tokens over the paged cache:
+ * row t at position p of its sequence attends cache rows j <= p, with a
+ * window (window > 0) only those with p - j < window or j < sinks (the first
+ * rows, kept visible). out[t] = sum_j softmax_j(scale * q . k_j) v_j, fp32
+ * accumulation, the probabilities rounded to dt before the product with v;
+ * zeros for a row that sees nothing. q as above (row stride ldq, head stride
+ * q_head_stride); out [T][n_q_heads * head_dim], row stride ld_out, the input
+ * of the O projection. max_q bounds the new tokens of one sequence; 1 is the
+ * decode step. n_q_heads / n_kv_heads an integer up to 16.
+ * A cache row that no row of its sequence sees (behind kv_len, outside every
+ * window) may hold anything. Rows that are seen must be finite where another
+ * row of the same sequence does not see them: 0 * infinity is not 0.
+ * workspace: ie_paged_attention_workspace_size() bytes, 16-byte aligned,
+ * needing no initialisation and no state between calls; calls that share one
+ * must not overlap on the GPU (one stream, or ordered streams, and not two
+ * captured graphs that may run at once). The same call gives the same bits
+ * every time; a row's last bits may depend on the other sequences of the
+ * batch, which decide how the work is divided. */
+size_t ie_paged_attention_workspace_size(void);
+int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_heads,
+                       const void* q, int64_t ldq, int64_t q_head_stride,
+                       const ie_paged_cache* cache, const int* page_table, int64_t ld_table, int max_pages,
+                       const int* q_start, const int* kv_len, int window, int sinks, float scale,
+                       void* out, int64_t ld_out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- a6 + a7: lm_head with fused greedy argmax --------------------------
  * Replaces lm_head (kernels/lm_head.cu:5-20) followed by sample_token_amax
  * (kernels/sampling.cu:54-58), for M rows at once.
@@ -320,6 +395,28 @@ int ie_lm_head_argmax_noalloc(ie_dtype dt, int M, int K, int V, int64_t vocab_of
  */
 int ie_argmax(ie_dtype dt, int M, int V, const void* logits, int64_t ld,
               int* idx_out, void* stream);
+
+/* ---- sampling ---------------------------------------------------------------
+ * No counterpart in the reference (greedy only). One token id for each of M
+ * rows of V logits (row stride ld; any alignment of the type), from device
+ * arrays of M entries. With the row's tokens in descending order of logit
+ * (equal logits: lowest id first) and w = exp((x - max) / temperature):
+ *   top_k  (NULL, <= 0 or >= V: off) keeps the first top_k;
+ *   top_p  (NULL or >= 1: off) keeps those whose mass before them is below
+ *          top_p times the mass of the top_k;
+ *   min_p  (NULL or <= 0: off) keeps those with w >= min_p;
+ * the first token is always kept. idx_out gets the first token whose running
+ * mass exceeds u times the kept mass (u in [0, 1); a larger u gives the last
+ * kept token), logprob_out (nullable) the log of its share of the kept mass.
+ * temperature (NULL: 1) not above 0, NaN included: the first token, logprob 0.
+ * Masses are 64-bit sums over the distinct values, so the ids do not depend
+ * on an order of summation. -infinity and NaN logits are never sampled;
+ * a row without others gives idx -1 and logprob -infinity. The tie order
+ * differs from ie_argmax's, which follows the reference's tree.
+ * V at most 524160 (IE_ERR_UNSUPPORTED above). */
+int ie_sample(ie_dtype dt, int M, int V, const void* logits, int64_t ld,
+              const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* u,
+              int* idx_out, float* logprob_out, void* stream);
 
 /* ---- e1: tensor-parallel exchange steps -------------------------------------
  * No counterpart in the reference (single GPU only). Megatron-style split of

@@ -18,6 +18,10 @@ on this path is the stream; these functions take `stream=` instead (default:
 torch's current stream). Failures raise IEError carrying the library status,
 where the reference would silently continue.
 
+The paged-cache operators and the sampler (no counterpart in the reference:
+PagedCache, qk_norm_rope_paged, paged_attention, sample) are in paged.py and
+offered here.
+
 There is no CPU path: every call goes to libinfengine_b200.so and raises if
 the library or a CUDA device is missing.
 """
@@ -63,6 +67,7 @@ EXPORTED_SYMBOLS = (
     "ie_qkv_ws",
     "ie_st_open", "ie_st_close", "ie_st_count", "ie_st_name", "ie_st_info", "ie_llama_load", "ie_llama_model_desc",
     "ie_llama_model_shard", "ie_llama_model_free",
+    "ie_qk_norm_rope_paged", "ie_paged_attention", "ie_paged_attention_workspace_size", "ie_sample",
 )
 
 
@@ -376,3 +381,17 @@ def sample_token_amax(d_logits, d_output, stream=None):
     V = d_logits.numel()
     _check(lib().ie_argmax(_dt(d_logits), 1, V, _ptr(d_logits), V, _ptr(d_output), _stream(stream)),
            "sample_token_amax")
+
+
+# ------------------------------------------- paged cache and sampling (paged.py)
+# torch is imported with the first use of one of these names, as everywhere above
+_PAGED = ("PagedCache", "paged_attention", "paged_attention_workspace", "paged_attention_workspace_bytes",
+          "qk_norm_rope_paged", "sample")
+
+
+def __getattr__(name):
+    if name in _PAGED:
+        from . import paged
+        globals().update({n: getattr(paged, n) for n in _PAGED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -6,6 +6,7 @@
 #include "gemm_tc.cuh"
 #include "attention.cuh"
 #include "norm.cuh"
+#include "paged_ops.cuh"
 
 using namespace ie;
 
@@ -61,13 +62,18 @@ int ie_device_status(int clear) {
   const int c = read_attn_status(clear != 0);
   const int d = read_norm_status(clear != 0);
   const int e = read_tca_status(clear != 0);
-  return a != IE_OK ? a : (b != IE_OK ? b : (c != IE_OK ? c : (d != IE_OK ? d : e)));
+  const int f = read_paged_attn_status(clear != 0);
+  const int g = read_paged_norm_status(clear != 0);
+  for (const int x : {a, b, c, d, e, f, g})
+    if (x != IE_OK) return x;
+  return IE_OK;
 }
 
 int ie_set_wait_limit_ns(unsigned long long ns) {
   if (ns > kMaxWaitNs) return IE_ERR_INVALID_ARG;
   const unsigned long long v = ns ? ns : kDefaultWaitNs;
-  const cudaError_t e[4] = {set_tc_wait_ns(v), set_skinny_wait_ns(v), set_attn_wait_ns(v), set_tca_wait_ns(v)};
+  const cudaError_t e[5] = {set_tc_wait_ns(v), set_skinny_wait_ns(v), set_attn_wait_ns(v), set_tca_wait_ns(v),
+                            set_paged_attn_wait_ns(v)};
   for (const cudaError_t x : e)
     if (x != cudaSuccess) return IE_ERR_LAUNCH;
   return IE_OK;

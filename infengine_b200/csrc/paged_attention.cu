@@ -1,0 +1,647 @@
+// Attention of new tokens over a paged cache: entry point, the kernel for few
+// rows, and the kernel that joins split tiles.
+//
+//   x_j = scale * q . k_j        keys j <= position with (position - j < window or j < sinks)
+//   o   = sum_j e^(x_j - m) v_j / sum_j e^(x_j - m)       zeros where no key is seen
+//
+// in one pass with a running maximum m (base 2, scale * log2 e folded into one
+// factor), fp32 throughout; p_j is rounded to the storage type for the tensor
+// cores and the sum takes the rounded values, so a rounding of p moves weight
+// between keys but not the total.
+//
+// few_rows_kernel (at most 16 (token, head) rows a tile: decode, verification
+// of a few draft tokens). What bounds it: a cache row of 512 bytes costs
+// 16 flop a byte, far below the tensor cores, so the cache's bytes over HBM do,
+// and for short contexts the latency of one chain (page entry, copy, scores,
+// softmax, values, join). A warp works alone on its own range of keys, 32 at a
+// time: its lane 0 keeps copies of the next key and value blocks in flight
+// into the warp's ring (TMA boxes of up to 32 rows of one page x 64
+// dimensions, 128-byte swizzle, conflict-free for ldmatrix), the products run
+// as m16n8k16 with the rows as M, and no barrier is shared between warps until
+// the four warps' outputs meet at the end. 96 KB of ring a CTA, two CTAs an SM:
+// 192 KB of copies in flight an SM, above the ~50 KB that HBM latency needs.
+//
+// A block's box is copied only if some row of the tile sees one of its keys, so
+// table entries outside the visible range are never followed; visible range's
+// edges inside a box are zeroed in shared memory before the product, so what a
+// page holds there (NaN included) does not reach a sum.
+#include <cstdio>
+#include <cstring>
+#include "ie_common.cuh"
+#include "paged_attention.cuh"
+#include "paged_ops.cuh"
+#include "norm.cuh"
+#include "tc_ptx.cuh"
+
+namespace ie {
+
+__device__ int g_paged_attn_status = 0;
+__device__ unsigned long long g_paged_attn_wait_ns = kDefaultWaitNs;
+
+namespace pa {
+namespace {
+
+using namespace tc;
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kKB = 32;           // keys of a warp's block
+constexpr int kMT = kRowsFew;
+constexpr int kRingBytes = 24576;  // a warp's ring
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT<T>::id == IE_DTYPE_F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT<T>::id == IE_DTYPE_BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t r) {
+  if constexpr (DT<T>::id == IE_DTYPE_BF16)
+    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&r));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_constant__ Args a) {
+  constexpr int kSlotBytes = kKB * D * 2;         // a key or value block: D / 64 halves of 32 rows x 128 bytes
+  constexpr int kSlots = kRingBytes / kSlotBytes;  // 3 (D = 128) or 6
+  constexpr int kHalf = kKB * 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t bars[kWarps * kSlots];
+  __shared__ Scan scan;
+  __shared__ float sm_m[kWarps][kMT], sm_l[kWarps][kMT];
+  __shared__ int abort_s;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps * kSlots; ++i) mbar_init(smem_u32(bars + i), 1);
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!find_piece<kMT, kKB, kThreads>(a, blockIdx.x, scan, &g_paged_attn_status)) return;
+  const Piece pc = scan.p;
+  const Seq sq = sequence(a, pc.b);
+  const int rows = sq.tokens * a.group;
+  const int row0 = pc.tile * kMT, nrows = min(kMT, rows - row0);
+  const int tok0 = row0 / a.group, tok1 = (row0 + nrows - 1) / a.group;
+  const Keys ks = tile_keys<kKB>(a, sq, tok0, tok1);
+  const int nb = ks.blocks();
+  const int p0 = (int)((int64_t)nb * pc.piece / pc.pieces), p1 = (int)((int64_t)nb * (pc.piece + 1) / pc.pieces);
+  const int j0 = p0 + (int)((int64_t)(p1 - p0) * warp / kWarps);
+  const int n = p0 + (int)((int64_t)(p1 - p0) * (warp + 1) / kWarps) - j0;
+
+  uint8_t* ring = smem + warp * kRingBytes;
+  const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(bars + warp * kSlots);
+  volatile int* abort_flag = &abort_s;
+  const int* table = a.b.page_table + (int64_t)pc.b * a.b.ld_table;
+  const int box = min(a.l.page_size, kKB), boxes = kKB / box;  // rows of a copy, copies of a block's half
+  const int per_batch = 32 / boxes;                            // blocks whose table entries a warp holds
+
+  auto box_seen = [&](int kb) { return kb < ks.hi && (kb + box > ks.lo || kb < ks.sink_end); };
+  // entry `lane` of the batch of blocks it0 ..: its page, -1 where no copy is made
+  auto load_entries = [&](int it0) {
+    const int it = it0 + lane / boxes;
+    if (it >= n) return -1;
+    const int kb = ks.block(j0 + it) * kKB + (lane % boxes) * box;
+    if (!box_seen(kb)) return -1;
+    const int page = table[kb >> a.l.page_log2];
+    if (page < 0 || page >= a.l.num_pages) {
+      atomicExch(&g_paged_attn_status, IE_ERR_INVALID_ARG);
+      return a.l.num_pages;  // outside the tensor map: zeros
+    }
+    return page;
+  };
+  int entries = load_entries(0), entries_next = load_entries(per_batch), batch = 0;
+  // copy i: keys of block i / 2 (even) or values (odd)
+  auto issue = [&](int i) {
+    const int it = i >> 1;
+    if (it >= n) return;
+    if (it >= batch + per_batch) {
+      batch += per_batch;
+      entries = entries_next;
+      entries_next = load_entries(batch + per_batch);
+    }
+    const int slot = i % kSlots;
+    const uint32_t dst = ring_u + slot * kSlotBytes, bar = bar_u + 8 * slot;
+    const int kb = ks.block(j0 + it) * kKB;
+    const CUtensorMap* map = (i & 1) ? &a.tmV : &a.tmK;
+    int pages[2];
+    pages[0] = __shfl_sync(0xffffffffu, entries, (it - batch) * boxes);
+    pages[1] = boxes == 2 ? __shfl_sync(0xffffffffu, entries, (it - batch) * boxes + 1) : -1;
+    if (lane == 0) {
+      mbar_expect_tx(bar, ((pages[0] >= 0) + (pages[1] >= 0)) * box * D * 2);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (pages[x] >= 0) {
+          const int r = (kb + x * box) & (a.l.page_size - 1);
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_4d(dst + h * kHalf + x * box * 128, map, bar, 64 * h, a.swap_rc ? pc.head : r,
+                        a.swap_rc ? r : pc.head, pages[x]);
+        }
+    }
+  };
+
+  // Q as A operands (rows lane / 4 and lane / 4 + 8)
+  const int g = lane >> 2, tq = lane & 3;
+  uint32_t qa[D / 16][4];
+  int pos[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = g + 8 * x;
+    const int tok = (row0 + r) / a.group;
+    pos[x] = sq.pos0 + tok;
+    const T* qr = static_cast<const T*>(a.q) + (int64_t)(sq.start + tok) * a.ldq +
+                  (int64_t)(pc.head * a.group + (row0 + r) % a.group) * a.hsq;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      qa[k][x] = r < nrows ? *reinterpret_cast<const uint32_t*>(qr + 16 * k + 2 * tq) : 0u;
+      qa[k][x + 2] = r < nrows ? *reinterpret_cast<const uint32_t*>(qr + 16 * k + 8 + 2 * tq) : 0u;
+    }
+  }
+  __syncthreads();  // the barriers are initialised
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) issue(i);
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int pos_min = sq.pos0 + tok0, pos_max = sq.pos0 + tok1;
+  auto wait = [&](int i) {
+    return mbar_wait(bar_u + 8 * (i % kSlots), (uint32_t)((i / kSlots) & 1), abort_flag, &g_paged_attn_status,
+                     &g_paged_attn_wait_ns);
+  };
+  int done = 0;  // copies waited for
+  bool ok = true;
+  for (int it = 0; it < n; ++it) {
+    const int kb = ks.block(j0 + it) * kKB;
+    // ---- scores
+    ok = __all_sync(0xffffffffu, wait(2 * it));
+    if (!ok) break;
+    float s[kKB / 8][4];
+#pragma unroll
+    for (int i = 0; i < kKB / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    {
+      const uint32_t base = ring_u + (2 * it % kSlots) * kSlotBytes;
+      const int key = ((lane >> 4) & 1) * 8 + (lane & 7), c = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int y = 0; y < kKB / 16; ++y) {
+          uint32_t b[4];
+          const int row = y * 16 + key, c16 = 2 * k + c;
+          ldsm4(base + (c16 >> 3) * kHalf + row * 128 + (((c16 & 7) ^ (row & 7)) << 4), b);
+          mma16816<T>(s[2 * y], qa[k], b[0], b[1]);
+          mma16816<T>(s[2 * y + 1], qa[k], b[2], b[3]);
+        }
+    }
+    __syncwarp();
+    issue(2 * it + kSlots);
+    done = 2 * it + 1;
+    // ---- softmax over the block: columns 8i + 2 tq + {0, 1}, rows g and g + 8
+#pragma unroll
+    for (int i = 0; i < kKB / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] *= a.scale_log2;
+    if (kb + kKB - 1 > pos_min || (a.window && (int64_t)pos_max - kb >= a.window)) {
+#pragma unroll
+      for (int i = 0; i < kKB / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = kb + 8 * i + 2 * tq + (e & 1), p = pos[e >> 1];
+          const bool seen = j <= p && j < ks.hi && (!a.window || p - j < a.window || j < a.sinks);
+          s[i][e] = seen ? s[i][e] : -INFINITY;
+        }
+    }
+    float mx[2] = {m[0], m[1]};
+#pragma unroll
+    for (int i = 0; i < kKB / 8; ++i) {
+      mx[0] = fmaxf(mx[0], fmaxf(s[i][0], s[i][1]));
+      mx[1] = fmaxf(mx[1], fmaxf(s[i][2], s[i][3]));
+    }
+    float base[2];
+    bool moved = false;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+      mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+      base[x] = mx[x] == -INFINITY ? 0.f : mx[x];
+      moved = moved || mx[x] != m[x];
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f = ex2(m[x] - base[x]);
+        l[x] *= f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][2 * x] *= f;
+          o[i][2 * x + 1] *= f;
+        }
+        m[x] = mx[x];
+      }
+    }
+    uint32_t pa[kKB / 16][4];
+#pragma unroll
+    for (int i = 0; i < kKB / 8; ++i) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t w = pack2<T>(ex2(s[i][2 * x] - base[x]), ex2(s[i][2 * x + 1] - base[x]));
+        const float2 r = unpack2<T>(w);
+        l[x] += r.x + r.y;
+        pa[i >> 1][2 * (i & 1) + x] = w;
+      }
+    }
+    // ---- values
+    ok = __all_sync(0xffffffffu, wait(2 * it + 1));
+    if (!ok) break;
+    uint8_t* vb = ring + ((2 * it + 1) % kSlots) * kSlotBytes;
+    if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
+      const int j = kb + lane;  // one row a lane
+      if (!(j < ks.hi && (j >= ks.lo || j < ks.sink_end))) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<uint4*>(vb + (c >> 3) * kHalf + lane * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this slot
+      __syncwarp();
+    }
+    {
+      const uint32_t vu = smem_u32(vb);
+      const int key = ((lane >> 3) & 1) * 8 + (lane & 7), c = lane >> 4;
+#pragma unroll
+      for (int y = 0; y < kKB / 16; ++y)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t b[4];
+          const int row = y * 16 + key, c16 = 2 * k + c;
+          ldsm4_t(vu + (c16 >> 3) * kHalf + row * 128 + (((c16 & 7) ^ (row & 7)) << 4), b);
+          mma16816<T>(o[2 * k], pa[y], b[0], b[1]);
+          mma16816<T>(o[2 * k + 1], pa[y], b[2], b[3]);
+        }
+    }
+    __syncwarp();
+    issue(2 * it + 1 + kSlots);
+    done = 2 * it + 2;
+  }
+  if (!ok) {
+    // copies in flight land before the CTA leaves (bounded; they always end)
+    const int issued = min(2 * n, done + kSlots);
+    for (int i = done; i < issued; ++i) {
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try(bar_u + 8 * (i % kSlots), (uint32_t)((i / kSlots) & 1)) && globaltimer() - t0 < kDrainWaitNs) {
+      }
+    }
+  }
+
+  // ---- the four warps meet: scale to the common maximum, add in warp order
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    if (tq == 0) {
+      sm_m[warp][g + 8 * x] = m[x];
+      sm_l[warp][g + 8 * x] = l[x];
+    }
+  }
+  __syncthreads();
+  if (abort_s) return;
+  float* acc = reinterpret_cast<float*>(ring);  // [16][D], this warp's
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = g + 8 * x;
+    float top = sm_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+    const float f = top == -INFINITY ? 0.f : ex2(m[x] - top);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+      *reinterpret_cast<float2*>(acc + r * D + ((8 * i + 2 * tq) ^ (8 * (r & 3)))) =
+          make_float2(o[i][2 * x] * f, o[i][2 * x + 1] * f);
+  }
+  __syncthreads();
+  const bool cut = pc.slot >= 0;
+  if (cut && (pc.slot >= a.slot_cap || pc.split >= a.split_cap)) return;
+  constexpr int kPer = kMT * D / kThreads;  // consecutive outputs of a thread
+  const int r = tid / (D / kPer), d0 = (tid % (D / kPer)) * kPer;
+  if (r < nrows) {
+    float top = sm_m[0][r], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += top == -INFINITY ? 0.f : sm_l[w][r] * ex2(sm_m[w][r] - top);
+    float v[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      float4 t4 = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * kRingBytes) +
+                                                          r * D + ((d0 + i) ^ (8 * (r & 3))));
+        t4.x += u.x; t4.y += u.y; t4.z += u.z; t4.w += u.w;
+      }
+      v[i] = t4.x; v[i + 1] = t4.y; v[i + 2] = t4.z; v[i + 3] = t4.w;
+    }
+    if (cut) {
+      float* po = a.part_o + ((int64_t)pc.slot * kMT + r) * D + d0;
+#pragma unroll
+      for (int i = 0; i < kPer; i += 4)
+        *reinterpret_cast<float4*>(po + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      if (d0 == 0) a.part_ml[(int64_t)pc.slot * kMT + r] = make_float2(top, sum);
+    } else {
+      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+      const int tok = (row0 + r) / a.group;
+      T* dst = static_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.ld_out +
+               (int64_t)(pc.head * a.group + (row0 + r) % a.group) * D + d0;
+#pragma unroll
+      for (int i = 0; i < kPer; i += 8) {
+        uint4 w;
+        w.x = pack2<T>(v[i] * inv, v[i + 1] * inv);
+        w.y = pack2<T>(v[i + 2] * inv, v[i + 3] * inv);
+        w.z = pack2<T>(v[i + 4] * inv, v[i + 5] * inv);
+        w.w = pack2<T>(v[i + 6] * inv, v[i + 7] * inv);
+        *reinterpret_cast<uint4*>(dst + i) = w;
+      }
+    }
+  }
+  if (cut && pc.piece == 0 && tid == 0) {
+    Split s = {};
+    s.slot0 = pc.slot;
+    s.pieces = pc.pieces;
+    s.token0 = sq.start;
+    s.rows = nrows;
+    s.head0 = pc.head * a.group;
+    s.row0 = row0;
+    a.splits[pc.split] = s;
+  }
+}
+
+// Joins a cut tile's pieces, one row a CTA: with M = max_s m_s, the output is
+// sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s in piece order. The four warps
+// take every fourth piece each, so that enough loads are in flight for the row
+// to cost one round trip for a few dozen pieces.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const Args a, int MT, int rows_most) {
+  constexpr int kV = D / 32;
+  __shared__ float red[4][D];
+  __shared__ float red_l[4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nkv = a.l.n_kv_heads;
+  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * rows_most;
+  for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
+    const Split sp = a.splits[x / rows_most];
+    const int r = (int)(x % rows_most);
+    if (r >= sp.rows) continue;  // the same for the whole block
+    auto at = [&](int s) { return ((int64_t)sp.slot0 + (int64_t)s * nkv) * MT + r; };
+    float top = -INFINITY;
+    for (int s = lane; s < sp.pieces; s += 32) top = fmaxf(top, a.part_ml[at(s)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float acc[kV] = {}, sum = 0.f;
+    if (top != -INFINITY) {
+#pragma unroll 4
+      for (int s = warp; s < sp.pieces; s += 4) {
+        const float2 ml = a.part_ml[at(s)];
+        const float f = ex2(ml.x - top);
+        sum += f * ml.y;
+        const float* po = a.part_o + at(s) * D + lane * kV;
+        float v[kV];
+        if constexpr (kV == 4) {
+          const float4 u = *reinterpret_cast<const float4*>(po);
+          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        } else {
+          const float2 u = *reinterpret_cast<const float2*>(po);
+          v[0] = u.x; v[1] = u.y;
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i) acc[i] += f * v[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kV; ++i) red[warp][lane * kV + i] = acc[i];
+    if (lane == 0) red_l[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+      const int d = 2 * threadIdx.x;
+      const float t = red_l[0] + red_l[1] + red_l[2] + red_l[3], inv = t > 0.f ? 1.0f / t : 0.f;
+      const float lo = (red[0][d] + red[1][d] + red[2][d] + red[3][d]) * inv;
+      const float hi = (red[0][d + 1] + red[1][d + 1] + red[2][d + 1] + red[3][d + 1]) * inv;
+      const int row = sp.row0 + r;
+      T* dst = static_cast<T*>(a.out) + (int64_t)(sp.token0 + row / a.group) * a.ld_out +
+               (int64_t)(sp.head0 + row % a.group) * D + d;
+      *reinterpret_cast<uint32_t*>(dst) = pack2<T>(lo, hi);
+    }
+    __syncthreads();
+  }
+}
+
+// A page's rows as boxes of 64 dimensions x `box` rows of one head and page,
+// zeros outside. The map lists row and head in the order of their strides.
+bool make_map(CUtensorMap* map, ie_dtype dt, const void* base, int D, const PagedLayout& l, int box, bool swap) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)(swap ? l.n_kv_heads : l.page_size),
+                        (cuuint64_t)(swap ? l.page_size : l.n_kv_heads), (cuuint64_t)l.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)(swap ? l.head_stride : l.row_stride) * 2,
+                           (cuuint64_t)(swap ? l.row_stride : l.head_stride) * 2, (cuuint64_t)l.page_stride * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)(swap ? 1 : box), (cuuint32_t)(swap ? box : 1), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t =
+      dt == IE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, t, 4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+template <typename K>
+int launch(K kernel, dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t st, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), args);
+  if (e != cudaSuccess) {
+    std::fprintf(stderr, "infengine_b200: paged attention launch failed: %s\n", cudaGetErrorString(e));
+    return IE_ERR_LAUNCH;
+  }
+  return IE_OK;
+}
+
+template <typename T, int D>
+int launch_few(Args& a, int64_t grid, cudaStream_t st) {
+  constexpr size_t kSmem = kWarps * kRingBytes + 1024;
+  auto kernel = few_rows_kernel<T, D>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return IE_ERR_LAUNCH;
+  static bool configured[64] = {};
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+      return IE_ERR_LAUNCH;
+    configured[dev] = true;
+  }
+  void* args[] = {&a};
+  return launch(kernel, dim3((unsigned)grid), kThreads, kSmem, pdl_launch_enabled() && a.b.T <= pdl_max_rows(), st,
+                args);
+}
+
+}  // namespace
+
+int launch_join(ie_dtype dt, int D, int MT, const Args& a, int rows, int64_t most, cudaStream_t st) {
+  const int64_t items = most * rows;
+  const unsigned grid = (unsigned)(items < 148 * 8 ? items : 148 * 8);
+  Args copy = a;
+  void* args[] = {&copy, &MT, &rows};
+  auto go = [&](auto kernel) { return launch(kernel, dim3(grid), 128, 0, pdl_launch_enabled(), st, args); };
+  if (dt == IE_DTYPE_F16) return D == 128 ? go(join_kernel<__half, 128>) : go(join_kernel<__half, 64>);
+  return D == 128 ? go(join_kernel<__nv_bfloat16, 128>) : go(join_kernel<__nv_bfloat16, 64>);
+}
+
+namespace {
+
+// workspace: number of cut tiles | their descriptions | (maximum, sum) | outputs
+constexpr int kCapSplits = kTargetFew > kTargetChunk ? kTargetFew : kTargetChunk;
+constexpr int64_t kSlotRowsFew = (int64_t)2 * kTargetFew * kRowsFew;
+constexpr int64_t kSlotRowsChunk = (int64_t)2 * kTargetChunk * kRowsChunk;
+constexpr int64_t kSlotRows = kSlotRowsFew > kSlotRowsChunk ? kSlotRowsFew : kSlotRowsChunk;
+constexpr size_t kOffSplits = 256;
+constexpr size_t kOffMl = kOffSplits + kCapSplits * sizeof(Split);
+constexpr size_t kOffO = kOffMl + kSlotRows * sizeof(float2);
+constexpr size_t kWorkspace = kOffO + kSlotRows * 128 * sizeof(float);
+static_assert(kOffMl % 16 == 0 && kOffO % 16 == 0, "alignment of the workspace's parts");
+
+}  // namespace
+}  // namespace pa
+
+int read_paged_attn_status(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_paged_attn_status, sizeof(int)) != cudaSuccess) return IE_ERR_LAUNCH;
+  if (clear && v) {
+    const int z = 0;
+    cudaMemcpyToSymbol(g_paged_attn_status, &z, sizeof(int));
+  }
+  return v;
+}
+
+cudaError_t set_paged_attn_wait_ns(unsigned long long ns) {
+  return cudaMemcpyToSymbol(g_paged_attn_wait_ns, &ns, sizeof(ns));
+}
+
+}  // namespace ie
+
+using namespace ie;
+
+extern "C" size_t ie_paged_attention_workspace_size(void) { return pa::kWorkspace; }
+
+extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_heads, const void* q, int64_t ldq,
+                                  int64_t q_head_stride, const ie_paged_cache* cache, const int* page_table,
+                                  int64_t ld_table, int max_pages, const int* q_start, const int* kv_len, int window,
+                                  int sinks, float scale, void* out, int64_t ld_out, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  using namespace pa;
+  if ((dt != IE_DTYPE_F16 && dt != IE_DTYPE_BF16) || n_q_heads <= 0 || max_q < 0 || window < 0 || sinks < 0)
+    return IE_ERR_INVALID_ARG;
+  int s = check_paged(cache, B, T, page_table, ld_table, max_pages, q_start, kv_len);
+  if (s) return s;
+  if (n_q_heads % cache->n_kv_heads) return IE_ERR_UNSUPPORTED;
+  const int D = cache->head_dim, group = n_q_heads / cache->n_kv_heads;
+  if (group > kRowsFew) return IE_ERR_UNSUPPORTED;
+  if (!(scale > -INFINITY && scale < INFINITY)) return IE_ERR_INVALID_ARG;
+  if (sinks && !window) return IE_ERR_INVALID_ARG;
+  if (B == 0 || T == 0 || max_q == 0) return IE_OK;
+  if (!q || !out || q_head_stride < D || ldq < 0 || ld_out < (int64_t)n_q_heads * D) return IE_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(out) || ldq % 8 || q_head_stride % 8 || ld_out % 8) return IE_ERR_ALIGNMENT;
+  if ((int64_t)max_q * group > INT_MAX - kRowsChunk || (int64_t)T * group > INT_MAX - kRowsChunk)
+    return IE_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < kWorkspace) return IE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return IE_ERR_ALIGNMENT;
+
+  Args a = {};
+  a.b = {q_start, kv_len, page_table, ld_table, B, T, max_pages};
+  a.l = paged_layout(cache);
+  a.q = q; a.ldq = ldq; a.hsq = q_head_stride;
+  a.out = out; a.ld_out = ld_out;
+  a.group = group; a.max_q = max_q; a.window = window; a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.swap_rc = cache->row_stride > cache->head_stride && cache->n_kv_heads > 1;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.n_split = reinterpret_cast<int*>(ws);
+  a.splits = reinterpret_cast<Split*>(ws + kOffSplits);
+  a.part_ml = reinterpret_cast<float2*>(ws + kOffMl);
+  a.part_o = reinterpret_cast<float*>(ws + kOffO);
+  a.split_cap = kCapSplits;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+
+  auto tiles = [&](int MT) {
+    const int64_t by_seq = (int64_t)B * (((int64_t)max_q * group + MT - 1) / MT);
+    const int64_t by_rows = (int64_t)T * group / MT + B;
+    return cache->n_kv_heads * (by_seq < by_rows ? by_seq : by_rows);
+  };
+  a.target = kTargetFew;
+  a.min_blocks = 4;
+  a.slot_cap = 2 * kTargetFew;
+  const int64_t most = tiles(kRowsFew), grid = most + kTargetFew;
+  if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
+  const int box = a.l.page_size < kKB ? a.l.page_size : kKB;
+  if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
+      !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
+    return IE_ERR_UNSUPPORTED;
+  if (dt == IE_DTYPE_F16) s = D == 128 ? launch_few<__half, 128>(a, grid, st) : launch_few<__half, 64>(a, grid, st);
+  else s = D == 128 ? launch_few<__nv_bfloat16, 128>(a, grid, st) : launch_few<__nv_bfloat16, 64>(a, grid, st);
+  if (s) return s;
+  const int rows = (int)((int64_t)max_q * group < kRowsFew ? (int64_t)max_q * group : kRowsFew);
+  return launch_join(dt, D, kRowsFew, a, rows, most < kTargetFew ? most : kTargetFew, st);
+}

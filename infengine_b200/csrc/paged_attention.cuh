@@ -1,0 +1,219 @@
+// Shared by the two paged-attention kernels (paged_attention.cu: few rows,
+// paged_attention_tc.cu: chunks): the arguments, the division of the work and
+// the partial results in the workspace.
+//
+// Work. A tile is up to MT rows of one sequence and KV head, a row one (token,
+// query head of the group) pair in that order, so that rows which share a
+// cache row share its load. The keys some row of the tile sees are covered by
+// blocks of KB keys (aligned; sink rows first). A tile with many blocks is cut
+// into S pieces of at most C blocks each, where C is chosen from the whole
+// batch so that the pieces fill the GPU; the pieces' unnormalised outputs,
+// maxima and sums meet in the workspace and a second kernel joins them in
+// piece order. All of it is computed on the device from the lengths, so a
+// captured graph follows them.
+#pragma once
+#include <cuda.h>
+#include "paged.cuh"
+
+namespace ie {
+namespace pa {
+
+struct Split {     // one tile that was cut, for the joining kernel
+  int slot0, pieces, token0, rows, head0, row0, pad0, pad1;
+};
+
+struct Args {
+  CUtensorMap tmK, tmV;  // (dim, row, head, page), or head before row where rows lie further apart
+  PagedBatch b;
+  PagedLayout l;
+  const void* q;
+  int64_t ldq, hsq;
+  void* out;
+  int64_t ld_out;
+  int group, max_q, window, sinks, swap_rc;
+  float scale_log2;
+  int target;     // pieces to aim at
+  int min_blocks; // smallest piece
+  int slot_cap, split_cap;
+  int* n_split;
+  Split* splits;
+  float2* part_ml;  // [slot][MT] (maximum in log2 units, sum)
+  float* part_o;    // [slot][MT][D]
+};
+
+// One sequence's extents after clamping to what the call was given.
+struct Seq {
+  int start, tokens, kv, pos0;  // first row of q, rows served, cache rows, position of the first row
+  bool bad;
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+  Seq s;
+  s.start = a.b.q_start[b];
+  const int64_t n = (int64_t)a.b.q_start[b + 1] - s.start;
+  const int kv = a.b.kv_len[b];
+  const int64_t cap = (int64_t)a.b.max_pages << a.l.page_log2;
+  s.bad = n < 0 || n > a.max_q || kv < 0 || kv > cap || s.start < 0 || (n > 0 && s.start + n > a.b.T);
+  s.kv = kv < 0 ? 0 : kv > cap ? (int)cap : kv;
+  int64_t serve = n < a.max_q ? n : a.max_q;
+  if (s.start < 0 || s.start >= a.b.T) serve = 0;
+  else if (s.start + serve > a.b.T) serve = a.b.T - s.start;
+  s.tokens = serve < 0 ? 0 : (int)serve;
+  const int64_t p = (int64_t)s.kv - (n < 0 ? 0 : n);
+  s.pos0 = (int)(p < -INT_MAX ? -INT_MAX : p);
+  return s;
+}
+template <int MT>
+__device__ __forceinline__ int tile_count(const Args& a, const Seq& s) {
+  return (int)(((int64_t)s.tokens * a.group + MT - 1) / MT);
+}
+// Most blocks any tile of the sequence can have.
+template <int MT, int KB>
+__device__ __forceinline__ int most_blocks(const Args& a, const Seq& s) {
+  const int all = (int)(((int64_t)s.kv + KB - 1) / KB);
+  if (!a.window) return all;
+  const int span = min(s.tokens, MT / a.group + 2);  // tokens of a tile
+  const int64_t w = ((int64_t)a.window + span) / KB + 2 + ((int64_t)a.sinks + KB - 1) / KB;
+  return (int)(w < all ? w : all);
+}
+
+// The keys of one tile: [lo, hi) and the sinks [0, sink_end), in blocks
+// 0 .. n_sink - 1 and first .. first + n_main - 1.
+struct Keys {
+  int lo, hi, sink_end, first, n_sink, n_main;
+  __device__ __forceinline__ int blocks() const { return n_sink + n_main; }
+  __device__ __forceinline__ int block(int j) const { return j < n_sink ? j : first + j - n_sink; }
+};
+template <int KB>
+__device__ __forceinline__ Keys tile_keys(const Args& a, const Seq& s, int tok0, int tok1) {  // tokens tok0 .. tok1
+  Keys k;
+  const int64_t hi = (int64_t)s.pos0 + tok1 + 1;
+  k.hi = (int)(hi < 0 ? 0 : hi < s.kv ? hi : s.kv);
+  k.lo = 0;
+  if (a.window) {
+    const int64_t lo = (int64_t)s.pos0 + tok0 - a.window + 1;
+    k.lo = (int)(lo < 0 ? 0 : lo < k.hi ? lo : k.hi);
+  }
+  k.sink_end = min(a.sinks, k.lo);
+  k.first = k.lo / KB;
+  k.n_main = k.hi > k.lo ? (k.hi + KB - 1) / KB - k.first : 0;
+  k.n_sink = min((k.sink_end + KB - 1) / KB, k.first);
+  if (k.n_main == 0) k.n_sink = 0;
+  return k;
+}
+
+struct Piece {
+  int b, head, tile, pieces, piece, slot, split;  // slot, split < 0: the tile is whole
+};
+
+// Scratch of find_piece.
+struct Scan {
+  long long w[3][32];
+  Piece p;
+  int found;
+};
+
+// Sum over the block / exclusive scan of three counts over the block.
+template <int THREADS>
+__device__ __forceinline__ void block_scan3(long long (&v)[3], long long (&total)[3], Scan& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x[3] = {v[0], v[1], v[2]};
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const long long u = __shfl_up_sync(0xffffffffu, x[j], o);
+      if (lane >= o) x[j] += u;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int j = 0; j < 3; ++j) sc.w[j][warp] = x[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    long long before = 0;
+    total[j] = 0;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < warp) before += sc.w[j][i];
+      total[j] += sc.w[j][i];
+    }
+    v[j] = before + x[j] - v[j];
+  }
+  __syncthreads();
+}
+
+// The piece a CTA serves; false when there are fewer pieces. Called by the
+// whole block. CTA 0 also writes the number of cut tiles.
+template <int MT, int KB, int THREADS>
+__device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, int* status) {
+  const int tid = threadIdx.x, nkv = a.l.n_kv_heads;
+  // blocks of the whole batch (each tile counted at its sequence's most)
+  long long u = 0;
+  for (int b = tid; b < a.b.B; b += THREADS) {
+    const Seq s = sequence(a, b);
+    u += (long long)tile_count<MT>(a, s) * nkv * most_blocks<MT, KB>(a, s);
+    if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+  if ((tid & 31) == 0) sc.w[0][tid >> 5] = u;
+  if (tid == 0) sc.found = 0;
+  __syncthreads();
+  u = 0;
+  for (int i = 0; i < THREADS / 32; ++i) u += sc.w[0][i];
+  __syncthreads();
+  long long c = (u + a.target - 1) / a.target;
+  if (c < a.min_blocks) c = a.min_blocks;
+  const int C = c > INT_MAX / 2 ? INT_MAX / 2 : (int)c;
+
+  long long run[3] = {0, 0, 0};  // pieces, slots, cut tiles so far
+  for (int b0 = 0; b0 < a.b.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    long long v[3] = {0, 0, 0}, total[3];
+    int tiles = 0, S = 1;
+    if (b < a.b.B) {
+      const Seq s = sequence(a, b);
+      tiles = tile_count<MT>(a, s);
+      S = max(1, (most_blocks<MT, KB>(a, s) + C - 1) / C);
+      v[0] = (long long)tiles * S * nkv;
+      v[1] = S > 1 ? v[0] : 0;
+      v[2] = S > 1 ? (long long)tiles * nkv : 0;
+    }
+    const long long mine = v[0];
+    block_scan3<THREADS>(v, total, sc);
+    const long long at = index - (run[0] + v[0]);
+    if (at >= 0 && at < mine) {
+      // the last (longest) tiles first; the heads of a piece next to one another
+      const int local = (int)at, h = local % nkv, r = local / nkv, i = tiles - 1 - r / S;
+      Piece p;
+      p.b = b;
+      p.head = h;
+      p.tile = i;
+      p.pieces = S;
+      p.piece = r % S;
+      p.slot = S > 1 ? (int)(run[1] + v[1] + (long long)(i * S + p.piece) * nkv + h) : -1;
+      p.split = S > 1 ? (int)(run[2] + v[2] + (long long)i * nkv + h) : -1;
+      sc.p = p;
+      sc.found = 1;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) run[j] += total[j];
+    if (index != 0 && run[0] > index) break;
+  }
+  if (index == 0 && tid == 0) *a.n_split = run[2] < a.split_cap ? (int)run[2] : a.split_cap;
+  __syncthreads();
+  return sc.found != 0;
+}
+
+// Joins the cut tiles' pieces (grid-stride over rows).
+int launch_join(ie_dtype dt, int D, int MT, const Args& a, int rows, int64_t most, cudaStream_t st);
+
+// Chunks of tokens on tcgen05 (paged_attention_tc.cu).
+int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, int rows, cudaStream_t st);
+
+constexpr int kRowsFew = 16;                  // MT of the few-rows kernel
+constexpr int kTargetFew = 148 * 8;           // its pieces
+constexpr int kRowsChunk = 256;               // MT of the chunk kernel
+constexpr int kTargetChunk = 148;
+
+}  // namespace pa
+}  // namespace ie
