@@ -29,7 +29,8 @@ CFLAGS = ARCH + [
 ]
 
 CORE_SOURCES = ["capi.cu", "skinny.cu", "gemm_tc.cu", "noalloc.cu", "comm.cu", "attention.cu", "p2p.cu", "norm.cu",
-                "engine.cu", "loader.cu", "attention_tc.cu", "paged_norm.cu", "paged_attention.cu", "sample.cu"]
+                "engine.cu", "loader.cu", "attention_tc.cu", "paged_norm.cu", "paged_attention.cu",
+                "paged_attention_tc.cu", "sample.cu"]
 DROPIN_SOURCES = ["dropin.cu"]
 
 LIB_CORE = PKG / "libinfengine_b200.so"

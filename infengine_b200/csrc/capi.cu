@@ -64,7 +64,8 @@ int ie_device_status(int clear) {
   const int e = read_tca_status(clear != 0);
   const int f = read_paged_attn_status(clear != 0);
   const int g = read_paged_norm_status(clear != 0);
-  for (const int x : {a, b, c, d, e, f, g})
+  const int h = read_paged_tc_status(clear != 0);
+  for (const int x : {a, b, c, d, e, f, g, h})
     if (x != IE_OK) return x;
   return IE_OK;
 }
@@ -72,8 +73,8 @@ int ie_device_status(int clear) {
 int ie_set_wait_limit_ns(unsigned long long ns) {
   if (ns > kMaxWaitNs) return IE_ERR_INVALID_ARG;
   const unsigned long long v = ns ? ns : kDefaultWaitNs;
-  const cudaError_t e[5] = {set_tc_wait_ns(v), set_skinny_wait_ns(v), set_attn_wait_ns(v), set_tca_wait_ns(v),
-                            set_paged_attn_wait_ns(v)};
+  const cudaError_t e[6] = {set_tc_wait_ns(v), set_skinny_wait_ns(v), set_attn_wait_ns(v), set_tca_wait_ns(v),
+                            set_paged_attn_wait_ns(v), set_paged_tc_wait_ns(v)};
   for (const cudaError_t x : e)
     if (x != cudaSuccess) return IE_ERR_LAUNCH;
   return IE_OK;

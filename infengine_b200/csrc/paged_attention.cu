@@ -630,6 +630,20 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
     const int64_t by_rows = (int64_t)T * group / MT + B;
     return cache->n_kv_heads * (by_seq < by_rows ? by_seq : by_rows);
   };
+  if ((int64_t)max_q * group > kRowsFew) {
+    a.target = kTargetChunk;
+    a.min_blocks = 2;
+    a.slot_cap = 2 * kTargetChunk;
+    const int64_t most = tiles(kRowsChunk), grid = most + kTargetChunk;
+    if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
+    const int box = a.l.page_size < 128 ? a.l.page_size : 128;
+    if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
+        !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
+      return IE_ERR_UNSUPPORTED;
+    if ((s = launch_chunks(dt, D, a, grid, st))) return s;
+    const int rows = (int)((int64_t)max_q * group < kRowsChunk ? (int64_t)max_q * group : kRowsChunk);
+    return launch_join(dt, D, kRowsChunk, a, rows, most < kTargetChunk ? most : kTargetChunk, st);
+  }
   a.target = kTargetFew;
   a.min_blocks = 4;
   a.slot_cap = 2 * kTargetFew;

@@ -208,7 +208,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
 int launch_join(ie_dtype dt, int D, int MT, const Args& a, int rows, int64_t most, cudaStream_t st);
 
 // Chunks of tokens on tcgen05 (paged_attention_tc.cu).
-int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, int rows, cudaStream_t st);
+int launch_chunks(ie_dtype dt, int D, Args& a, int64_t grid, cudaStream_t st);
 
 constexpr int kRowsFew = 16;                  // MT of the few-rows kernel
 constexpr int kTargetFew = 148 * 8;           // its pieces

@@ -8,7 +8,9 @@ namespace ie {
 // bounded wait for a copy or an MMA gave up.
 int read_paged_norm_status(bool clear);
 int read_paged_attn_status(bool clear);
+int read_paged_tc_status(bool clear);
 // Sets this device's limit of the kernels' bounded waits (current device).
 cudaError_t set_paged_attn_wait_ns(unsigned long long ns);
+cudaError_t set_paged_tc_wait_ns(unsigned long long ns);
 
 }  // namespace ie

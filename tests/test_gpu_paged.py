@@ -54,13 +54,16 @@ CHUNKS = [
     ([16], [16]), ([17], [17]), ([64], [64]), ([65], [200]), ([100], [1000]), ([128], [128]), ([129], [129]),
     ([255], [300]), ([256], [256]), ([257], [700]), ([300, 1, 0, 33], [300, 900, 20, 64]), ([1, 500], [2000, 511]),
     ([40], [11]),
+    ([2100], [2100]), ([900, 1500], [3500, 1501]),  # more tiles than SMs: whole ranges of many blocks
 ]
 
 
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("q_lens,kv_lens", CHUNKS)
 def test_attention_chunks(ie, cuda, dt, q_lens, kv_lens):
-    check_attention(ie, cuda, ref.make_batch(q_lens, kv_lens, dt=dt, seed=q_lens[0], spare_rows=5))
+    heads = 8 if max(q_lens) < 900 else 20
+    check_attention(ie, cuda, ref.make_batch(q_lens, kv_lens, heads=heads, kv_heads=heads // 4, dt=dt,
+                                             seed=q_lens[0], spare_rows=5))
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (6, 2), (5, 5), (8, 1), (16, 1), (14, 2), (32, 8)])
