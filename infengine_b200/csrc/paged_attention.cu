@@ -57,6 +57,9 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -117,16 +120,18 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   __shared__ int abort_s;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) {
+  if (tid == 32) {
     for (int i = 0; i < kWarps * kSlots; ++i) mbar_init(smem_u32(bars + i), 1);
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&a.tmK);
+    prefetch_map(&a.tmV);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (!find_piece<kMT, kKB, kThreads>(a, blockIdx.x, scan, &g_paged_attn_status)) return;
+  if (!find_piece<kKB, kThreads, false>(a, blockIdx.x, scan, &g_paged_attn_status)) return;
   const Piece pc = scan.p;
-  const Seq sq = sequence(a, pc.b);
+  const Seq sq = scan.seq;
   const int rows = sq.tokens * a.group;
   const int row0 = pc.tile * kMT, nrows = min(kMT, rows - row0);
   const int tok0 = row0 / a.group, tok1 = (row0 + nrows - 1) / a.group;
@@ -428,8 +433,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
 // take every fourth piece each, so that enough loads are in flight for the row
 // to cost one round trip for a few dozen pieces.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const Args a, int MT, int rows_most) {
-  constexpr int kV = D / 32;
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a, int rows_most) {
+  constexpr int kV = D / 32, MT = kMT;
   __shared__ float red[4][D];
   __shared__ float red_l[4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -483,6 +488,8 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, int MT, int row
   }
 }
 
+int launch_join(ie_dtype dt, int D, Args& a, int rows, int64_t most, cudaStream_t st);
+
 // A page's rows as boxes of 64 dimensions x `box` rows of one head and page,
 // zeros outside. The map lists row and head in the order of their strides.
 bool make_map(CUtensorMap* map, ie_dtype dt, const void* base, int D, const PagedLayout& l, int box, bool swap) {
@@ -497,6 +504,22 @@ bool make_map(CUtensorMap* map, ie_dtype dt, const void* base, int D, const Page
   const CUtensorMapDataType t =
       dt == IE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   return fn(map, t, 4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+// The queries as boxes of 64 dimensions x the heads of a group x `tokens`.
+bool make_q_map(CUtensorMap* map, ie_dtype dt, const void* q, int D, int T, int heads, int64_t ld, int64_t hs,
+                int group, int tokens) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)(T > 1 ? ld : D) * 2};
+  cuuint32_t boxes[3] = {64, (cuuint32_t)group, (cuuint32_t)tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType t =
+      dt == IE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(map, t, 3, const_cast<void*>(q), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
          CUDA_SUCCESS;
 }
@@ -538,19 +561,14 @@ int launch_few(Args& a, int64_t grid, cudaStream_t st) {
                 args);
 }
 
-}  // namespace
-
-int launch_join(ie_dtype dt, int D, int MT, const Args& a, int rows, int64_t most, cudaStream_t st) {
+int launch_join(ie_dtype dt, int D, Args& a, int rows, int64_t most, cudaStream_t st) {
   const int64_t items = most * rows;
   const unsigned grid = (unsigned)(items < 148 * 8 ? items : 148 * 8);
-  Args copy = a;
-  void* args[] = {&copy, &MT, &rows};
+  void* args[] = {&a, &rows};
   auto go = [&](auto kernel) { return launch(kernel, dim3(grid), 128, 0, pdl_launch_enabled(), st, args); };
   if (dt == IE_DTYPE_F16) return D == 128 ? go(join_kernel<__half, 128>) : go(join_kernel<__half, 64>);
   return D == 128 ? go(join_kernel<__nv_bfloat16, 128>) : go(join_kernel<__nv_bfloat16, 64>);
 }
-
-namespace {
 
 // workspace: number of cut tiles | their descriptions | (maximum, sum) | outputs
 constexpr int kCapSplits = kTargetFew > kTargetChunk ? kTargetFew : kTargetChunk;
@@ -602,7 +620,7 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   if (!(scale > -INFINITY && scale < INFINITY)) return IE_ERR_INVALID_ARG;
   if (sinks && !window) return IE_ERR_INVALID_ARG;
   if (B == 0 || T == 0 || max_q == 0) return IE_OK;
-  if (!q || !out || q_head_stride < D || ldq < 0 || ld_out < (int64_t)n_q_heads * D) return IE_ERR_INVALID_ARG;
+  if (!q || !out || q_head_stride < D || (T > 1 ? ldq < D : ldq < 0) || ld_out < (int64_t)n_q_heads * D) return IE_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(out) || ldq % 8 || q_head_stride % 8 || ld_out % 8) return IE_ERR_ALIGNMENT;
   if ((int64_t)max_q * group > INT_MAX - kRowsChunk || (int64_t)T * group > INT_MAX - kRowsChunk)
     return IE_ERR_UNSUPPORTED;
@@ -625,37 +643,35 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   a.split_cap = kCapSplits;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
-  auto tiles = [&](int MT) {
-    const int64_t by_seq = (int64_t)B * (((int64_t)max_q * group + MT - 1) / MT);
-    const int64_t by_rows = (int64_t)T * group / MT + B;
+  // most tiles a batch of these extents can have
+  auto tiles = [&](int rows) {
+    const int64_t by_seq = (int64_t)B * (((int64_t)max_q * group + rows - 1) / rows);
+    const int64_t by_rows = (int64_t)T * group / rows + B;
     return cache->n_kv_heads * (by_seq < by_rows ? by_seq : by_rows);
   };
-  if ((int64_t)max_q * group > kRowsFew) {
+  const bool few = (int64_t)max_q * group <= kRowsFew;
+  const int keys = few ? kKB : 64, box = a.l.page_size < keys ? a.l.page_size : keys;
+  if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
+      !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
+    return IE_ERR_UNSUPPORTED;
+  if (!few) {
+    a.lane_rows = kRowsChunk / 2 / group * group;
+    a.tile_rows = 2 * a.lane_rows;
     a.target = kTargetChunk;
-    a.min_blocks = 2;
+    a.min_blocks = 4;
     a.slot_cap = 2 * kTargetChunk;
-    const int64_t most = tiles(kRowsChunk), grid = most + kTargetChunk;
-    if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
-    const int box = a.l.page_size < 128 ? a.l.page_size : 128;
-    if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
-        !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
+    if (!make_q_map(&a.tmQ, dt, q, D, T, n_q_heads, ldq, q_head_stride, group, kRowsChunk / 2 / group))
       return IE_ERR_UNSUPPORTED;
-    if ((s = launch_chunks(dt, D, a, grid, st))) return s;
-    const int rows = (int)((int64_t)max_q * group < kRowsChunk ? (int64_t)max_q * group : kRowsChunk);
-    return launch_join(dt, D, kRowsChunk, a, rows, most < kTargetChunk ? most : kTargetChunk, st);
+    return launch_chunks(dt, D, a, tiles(a.tile_rows), st);
   }
+  a.tile_rows = kRowsFew;
   a.target = kTargetFew;
   a.min_blocks = 4;
   a.slot_cap = 2 * kTargetFew;
   const int64_t most = tiles(kRowsFew), grid = most + kTargetFew;
   if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
-  const int box = a.l.page_size < kKB ? a.l.page_size : kKB;
-  if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
-      !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
-    return IE_ERR_UNSUPPORTED;
   if (dt == IE_DTYPE_F16) s = D == 128 ? launch_few<__half, 128>(a, grid, st) : launch_few<__half, 64>(a, grid, st);
   else s = D == 128 ? launch_few<__nv_bfloat16, 128>(a, grid, st) : launch_few<__nv_bfloat16, 64>(a, grid, st);
   if (s) return s;
-  const int rows = (int)((int64_t)max_q * group < kRowsFew ? (int64_t)max_q * group : kRowsFew);
-  return launch_join(dt, D, kRowsFew, a, rows, most < kTargetFew ? most : kTargetFew, st);
+  return launch_join(dt, D, a, max_q * group, most < kTargetFew ? most : kTargetFew, st);
 }

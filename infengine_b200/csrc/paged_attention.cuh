@@ -2,9 +2,9 @@
 // paged_attention_tc.cu: chunks): the arguments, the division of the work and
 // the partial results in the workspace.
 //
-// Work. A tile is up to MT rows of one sequence and KV head, a row one (token,
-// query head of the group) pair in that order, so that rows which share a
-// cache row share its load. The keys some row of the tile sees are covered by
+// Work. A tile is up to tile_rows rows of one sequence and KV head, a row one
+// (token, query head of the group) pair in that order, so that rows which
+// share a cache row share its load. The keys some row of the tile sees are covered by
 // blocks of KB keys (aligned; sink rows first). A tile with many blocks is cut
 // into S pieces of at most C blocks each, where C is chosen from the whole
 // batch so that the pieces fill the GPU; the pieces' unnormalised outputs,
@@ -24,6 +24,7 @@ struct Split {     // one tile that was cut, for the joining kernel
 
 struct Args {
   CUtensorMap tmK, tmV;  // (dim, row, head, page), or head before row where rows lie further apart
+  CUtensorMap tmQ;       // (dim, head, token); chunk kernel
   PagedBatch b;
   PagedLayout l;
   const void* q;
@@ -31,14 +32,16 @@ struct Args {
   void* out;
   int64_t ld_out;
   int group, max_q, window, sinks, swap_rc;
+  int tile_rows;  // rows of a tile
+  int lane_rows;  // chunk kernel: rows of its lane, whole tokens (a tile is two lanes)
   float scale_log2;
   int target;     // pieces to aim at
   int min_blocks; // smallest piece
   int slot_cap, split_cap;
   int* n_split;
   Split* splits;
-  float2* part_ml;  // [slot][MT] (maximum in log2 units, sum)
-  float* part_o;    // [slot][MT][D]
+  float2* part_ml;  // [slot][row] (maximum in log2 units, sum)
+  float* part_o;    // few rows: [slot][16][D]; chunks: [slot][8 warps][D / 4][32 rows][4]
 };
 
 // One sequence's extents after clamping to what the call was given.
@@ -62,16 +65,15 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   s.pos0 = (int)(p < -INT_MAX ? -INT_MAX : p);
   return s;
 }
-template <int MT>
 __device__ __forceinline__ int tile_count(const Args& a, const Seq& s) {
-  return (int)(((int64_t)s.tokens * a.group + MT - 1) / MT);
+  return (s.tokens * a.group + a.tile_rows - 1) / a.tile_rows;  // the host checked the range
 }
 // Most blocks any tile of the sequence can have.
-template <int MT, int KB>
+template <int KB>
 __device__ __forceinline__ int most_blocks(const Args& a, const Seq& s) {
-  const int all = (int)(((int64_t)s.kv + KB - 1) / KB);
+  const int all = s.kv / KB + (s.kv % KB != 0);
   if (!a.window) return all;
-  const int span = min(s.tokens, MT / a.group + 2);  // tokens of a tile
+  const int span = min(s.tokens, a.tile_rows / a.group + 2);  // tokens of a tile
   const int64_t w = ((int64_t)a.window + span) / KB + 2 + ((int64_t)a.sinks + KB - 1) / KB;
   return (int)(w < all ? w : all);
 }
@@ -109,6 +111,7 @@ struct Piece {
 struct Scan {
   long long w[3][32];
   Piece p;
+  Seq seq;
   int found;
 };
 
@@ -141,16 +144,113 @@ __device__ __forceinline__ void block_scan3(long long (&v)[3], long long (&total
   __syncthreads();
 }
 
-// The piece a CTA serves; false when there are fewer pieces. Called by the
-// whole block. CTA 0 also writes the number of cut tiles.
-template <int MT, int KB, int THREADS>
+// Blocks of a piece, for u blocks in the batch (each tile counted at its
+// sequence's most).
+__device__ __forceinline__ int piece_blocks(const Args& a, long long u) {
+  long long c = u <= INT_MAX ? ((int)u - 1) / a.target + 1 : (u - 1) / a.target + 1;
+  if (c < a.min_blocks) c = a.min_blocks;
+  return c > INT_MAX / 2 ? INT_MAX / 2 : (int)c;
+}
+
+// Piece `at` of a sequence of `tiles` tiles in S pieces each: the last
+// (longest) tiles first, the heads of a piece next to one another.
+__device__ __forceinline__ Piece piece_at(const Args& a, int b, int tiles, int S, int at, int slots, int splits) {
+  const int nkv = a.l.n_kv_heads, r = at / nkv;
+  Piece p;
+  p.b = b;
+  p.head = at - r * nkv;
+  p.tile = tiles - 1 - (S > 1 ? r / S : r);
+  p.pieces = S;
+  p.piece = S > 1 ? r % S : 0;
+  p.slot = S > 1 ? slots + (p.tile * S + p.piece) * nkv + p.head : -1;
+  p.split = S > 1 ? splits + p.tile * nkv + p.head : -1;
+  return p;
+}
+
+// Blocks of a piece for a kernel of one CTA an SM, where whole waves count:
+// lane k - 1 weighs cutting the longest tile into k pieces of C = most / k
+// blocks. With P pieces of A blocks on average, W = ceil(P / SMs) waves cost
+// W (A + o) + C - A blocks, o the start and end of a piece in blocks (about
+// kWhole; kCut with the partial results' way through memory).
+constexpr int kWhole = 5, kCut = 9;
+__device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_heads, int most) {
+  const int k = (threadIdx.x & 31) + 1;
+  const int longest = __reduce_max_sync(0xffffffffu, most);
+  const int C = max((longest - 1) / k + 1, 1);
+  long long pieces = 0, cut = 0, blocks = 0;
+  for (int b = 0; b < a.b.B; ++b) {
+    const int t = __shfl_sync(0xffffffffu, tiles_heads, b), n = __shfl_sync(0xffffffffu, most, b);
+    const int S = n > C ? (n - 1) / C + 1 : 1;
+    pieces += (long long)t * S;
+    cut += S > 1 ? (long long)t * S : 0;
+    blocks += (long long)t * n;
+  }
+  const float avg = pieces ? (float)blocks / (float)pieces : 0.f;
+  const float waves = (float)((pieces + a.target - 1) / a.target);
+  float cost = waves * (avg + (cut ? kCut : kWhole)) + (float)C - avg;
+  if (cut > a.slot_cap || (k > 1 && C < a.min_blocks)) cost = INFINITY;
+  float least = cost;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  const int who = __ffs(__ballot_sync(0xffffffffu, cost == least)) - 1;
+  return __shfl_sync(0xffffffffu, C, max(who, 0));
+}
+
+// The piece a CTA serves and its sequence, in sc; false when there are fewer
+// pieces. Called by the whole block. CTA 0 also writes the number of cut tiles.
+template <int KB, int THREADS, bool kByWaves>
 __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, int* status) {
   const int tid = threadIdx.x, nkv = a.l.n_kv_heads;
-  // blocks of the whole batch (each tile counted at its sequence's most)
+  if (a.b.B <= 32) {
+    // one warp, one sequence a lane, one round trip to the lengths
+    if (tid < 32) {
+      Seq s = {};
+      int tiles = 0, most = 0;
+      if (tid < a.b.B) {
+        s = sequence(a, tid);
+        tiles = tile_count(a, s);
+        most = most_blocks<KB>(a, s);
+        if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
+      }
+      int C;
+      if constexpr (kByWaves) {
+        C = piece_blocks_by_waves(a, tiles * nkv, most);
+      } else {
+        long long u = (long long)tiles * nkv * most;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        C = piece_blocks(a, u);
+      }
+      const int S = most > C ? (most - 1) / C + 1 : 1;
+      // a count past the grid's range cannot be asked for: the host bounds the pieces
+      const int mine = (int)min((long long)tiles * S * nkv, 1LL << 25);
+      int x = mine, y = S > 1 ? mine : 0, z = S > 1 ? tiles * nkv : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int ux = __shfl_up_sync(0xffffffffu, x, o), uy = __shfl_up_sync(0xffffffffu, y, o),
+                  uz = __shfl_up_sync(0xffffffffu, z, o);
+        if (tid >= o) {
+          x += ux;
+          y += uy;
+          z += uz;
+        }
+      }
+      const bool hit = index >= x - mine && index < x;
+      if (hit) {
+        sc.p = piece_at(a, tid, tiles, S, index - (x - mine), y - (S > 1 ? mine : 0), z - (S > 1 ? tiles * nkv : 0));
+        sc.seq = s;
+      }
+      const unsigned any = __ballot_sync(0xffffffffu, hit);
+      if (tid == 0) sc.found = any != 0;
+      if (tid == 31 && index == 0) *a.n_split = min(z, a.split_cap);
+    }
+    __syncthreads();
+    return sc.found != 0;
+  }
   long long u = 0;
   for (int b = tid; b < a.b.B; b += THREADS) {
     const Seq s = sequence(a, b);
-    u += (long long)tile_count<MT>(a, s) * nkv * most_blocks<MT, KB>(a, s);
+    u += (long long)tile_count(a, s) * nkv * most_blocks<KB>(a, s);
     if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
   }
 #pragma unroll
@@ -161,19 +261,18 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
   u = 0;
   for (int i = 0; i < THREADS / 32; ++i) u += sc.w[0][i];
   __syncthreads();
-  long long c = (u + a.target - 1) / a.target;
-  if (c < a.min_blocks) c = a.min_blocks;
-  const int C = c > INT_MAX / 2 ? INT_MAX / 2 : (int)c;
-
+  const int C = piece_blocks(a, u);
   long long run[3] = {0, 0, 0};  // pieces, slots, cut tiles so far
   for (int b0 = 0; b0 < a.b.B; b0 += THREADS) {
     const int b = b0 + tid;
     long long v[3] = {0, 0, 0}, total[3];
     int tiles = 0, S = 1;
+    Seq s = {};
     if (b < a.b.B) {
-      const Seq s = sequence(a, b);
-      tiles = tile_count<MT>(a, s);
-      S = max(1, (most_blocks<MT, KB>(a, s) + C - 1) / C);
+      s = sequence(a, b);
+      const int most = most_blocks<KB>(a, s);
+      tiles = tile_count(a, s);
+      S = most > C ? (most - 1) / C + 1 : 1;
       v[0] = (long long)tiles * S * nkv;
       v[1] = S > 1 ? v[0] : 0;
       v[2] = S > 1 ? (long long)tiles * nkv : 0;
@@ -182,17 +281,8 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
     block_scan3<THREADS>(v, total, sc);
     const long long at = index - (run[0] + v[0]);
     if (at >= 0 && at < mine) {
-      // the last (longest) tiles first; the heads of a piece next to one another
-      const int local = (int)at, h = local % nkv, r = local / nkv, i = tiles - 1 - r / S;
-      Piece p;
-      p.b = b;
-      p.head = h;
-      p.tile = i;
-      p.pieces = S;
-      p.piece = r % S;
-      p.slot = S > 1 ? (int)(run[1] + v[1] + (long long)(i * S + p.piece) * nkv + h) : -1;
-      p.split = S > 1 ? (int)(run[2] + v[2] + (long long)i * nkv + h) : -1;
-      sc.p = p;
+      sc.p = piece_at(a, b, tiles, S, (int)at, (int)(run[1] + v[1]), (int)(run[2] + v[2]));
+      sc.seq = s;
       sc.found = 1;
     }
 #pragma unroll
@@ -204,15 +294,13 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
   return sc.found != 0;
 }
 
-// Joins the cut tiles' pieces (grid-stride over rows).
-int launch_join(ie_dtype dt, int D, int MT, const Args& a, int rows, int64_t most, cudaStream_t st);
+// Chunks of tokens on tcgen05 (paged_attention_tc.cu), with the joining of
+// their pieces. most_tiles: an upper bound of the batch's tiles.
+int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, cudaStream_t st);
 
-// Chunks of tokens on tcgen05 (paged_attention_tc.cu).
-int launch_chunks(ie_dtype dt, int D, Args& a, int64_t grid, cudaStream_t st);
-
-constexpr int kRowsFew = 16;                  // MT of the few-rows kernel
-constexpr int kTargetFew = 148 * 8;           // its pieces
-constexpr int kRowsChunk = 256;               // MT of the chunk kernel
+constexpr int kRowsFew = 16;         // tile_rows of the few-rows kernel
+constexpr int kTargetFew = 148 * 8;  // its pieces
+constexpr int kRowsChunk = 256;      // tile_rows of the chunk kernel, at most
 constexpr int kTargetChunk = 148;
 
 }  // namespace pa

@@ -3,10 +3,10 @@
 // the few-rows kernel takes.
 //
 // One CTA serves a piece: up to 256 (token, head) rows of one KV head, as two
-// lanes of 128 rows (one TMEM lane a row), over a range of 128-key blocks.
-// Both lanes use a key or value block from shared memory once it is there, so
-// L2 sees half the traffic of 128-row tiles, and while one lane's softmax runs
-// on its warps the tensor cores work for the other.
+// lanes of up to 128 rows (one TMEM lane a row; whole tokens, so 126 rows in
+// groups of 3), over a range of 64-key blocks. Both lanes use a key or value
+// block from shared memory once it is there, so L2 sees half the traffic of
+// 128-row tiles.
 //
 //   S = Q K^T  (fp32, TMEM)  ->  p = 2^(s c - m), c = scale log2 e  ->  O += P V
 //
@@ -17,25 +17,34 @@
 // sum takes the unrounded values.
 //
 // What bounds it: 128 x 128 scores cost 1024 cycles of tensor work (D = 128)
-// and 1024 cycles of exponentials (16 a cycle and SM), so the two are balanced
-// at best and the softmax chain has to stay off the tensor cores' path.
+// and 1024 cycles of exponentials on the special-function unit (16 a cycle and
+// SM). Each lane has two 64-key score buffers, so its next scores are ready
+// when its softmax is done with the last, and neither the tensor cores nor the
+// softmax wait for the other's latency: with one 128-key buffer a lane the
+// chain scores -> softmax -> product took 4900 cycles a 128-key block. A share
+// of the exponentials runs as a polynomial on the FMA pipes instead.
 //
-// TMEM columns: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 +
-// D); P overwrites the first 64 columns of the S it came from. Shared memory:
-// the two Q tiles, a ring of 5 key / value blocks (10 of D = 64). Operands are
-// 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K K-major, V
-// MN-major as it arrives.
+// TMEM columns: lane i's scores [128 i, 128 i + 64) and [128 i + 64, 128 i +
+// 128), O_i [256 + 128 i, + D); P overwrites the first 32 columns of the scores
+// it came from. Shared memory: the two Q tiles, a ring of key / value blocks.
+// Operands are 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K
+// K-major, V MN-major as it arrives.
 //
-// Warp roles: 0 copies (TMA boxes of up to 128 rows of one page; the lanes
-// hold the next table entries), 1 issues MMAs, 2 zeroes value rows that no row
-// of the tile sees (range edges inside a block; what the page holds there may
-// be NaN), 4-7 and 8-11 the lanes' softmax and epilogue. Every mbarrier wait is
-// bounded: on expiry IE_ERR_TIMEOUT is recorded, all roles leave their loops,
-// and MMAs and copies in flight are waited for before TMEM is freed.
+// Warp roles: 0 copies (Q, then TMA boxes of up to 64 rows of one page; the
+// lanes hold the next table entries), 1 and 3 issue the two lanes' MMAs (a
+// barrier wait costs an issuing warp about 110 cycles even when it is over,
+// and one warp for both lanes spent 2600 cycles a step on them), 2 zeroes value
+// rows that no row of the tile sees (range edges inside a block; what the page
+// holds there may be NaN), 4-7 and 8-11 the lanes' softmax and epilogue. Every
+// mbarrier wait is bounded: on expiry IE_ERR_TIMEOUT is recorded, all roles
+// leave their loops, and MMAs and copies in flight are waited for before TMEM
+// is freed.
 #include <cstdio>
+#include <type_traits>
 #include "ie_common.cuh"
 #include "paged_attention.cuh"
 #include "paged_ops.cuh"
+#include "norm.cuh"
 #include "tc_ptx.cuh"
 
 namespace ie {
@@ -48,19 +57,23 @@ namespace {
 
 using namespace tc;
 
-constexpr int kKB = 128;             // keys of a block
-constexpr int kMT = kRowsChunk;      // rows of a tile: two lanes of 128
+constexpr int kKB = 64;              // keys of a block
 constexpr int kThreads = 384;
 constexpr float kLazy = 8.0f;        // log2 of the growth of a row's maximum that O tolerates
 
 template <int D>
 struct Cfg {
-  static constexpr int kTile = kKB * D * 2;                   // one Q lane, key or value block
-  static constexpr int kHalf = kKB * 128;                     // its 64-dimension halves
-  static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kOffRing = 2 * kTile;
+  static constexpr int kQTile = 128 * D * 2;                  // a lane's queries
+  static constexpr int kQHalf = 128 * 128;                    // their 64-dimension halves
+  static constexpr int kTile = kKB * D * 2;                   // a key or value block
+  static constexpr int kHalf = kKB * 128;
+  static constexpr int kStages = 10;
+  static constexpr int kOffRing = 2 * kQTile;
   static constexpr int kOffBars = kOffRing + kStages * kTile;
   static constexpr int kSmem = kOffBars + 512 + 1024;         // + alignment slack
+  // Of 8 pairs of exponentials, those on the FMA pipes. D = 64 has half the
+  // tensor work, so there the special-function unit is the bound.
+  static constexpr int kPoly = 2;
 };
 static_assert(Cfg<128>::kSmem <= 227 * 1024 - 1024, "shared memory per CTA");
 
@@ -78,6 +91,64 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// ---- two fp32 values at a time
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// (2^a, 2^b) on the FMA pipes, for values up to 2^22: the nearest integer n by
+// adding 1.5 * 2^23, 2^f for the rest f in [-1/2, 1/2] by the polynomial of
+// degree 5 of least relative error (2^-23.7, 2^-22.1 as evaluated), n added to
+// the exponent field. Values below -126 count as -126.
+__device__ __forceinline__ void ex2_poly2(float& a, float& b) {
+  const uint64_t x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const float big = 12582912.0f;
+  const uint64_t r = add2(x, pair(big, big));
+  const uint64_t f = fma2(add2(r, pair(-big, -big)), pair(-1.0f, -1.0f), x);
+  auto c = [](float v) { return pair(v, v); };
+  uint64_t p = fma2(c(1.3276472e-3f), f, c(9.675541e-3f));
+  p = fma2(p, f, c(5.550713e-2f));
+  p = fma2(p, f, c(2.4022120e-1f));
+  p = fma2(p, f, c(6.9314694e-1f));
+  p = fma2(p, f, c(1.0000001f));
+  float r0, r1, p0, p1;
+  split(r, r0, r1);
+  split(p, p0, p1);
+  a = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+  b = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+}
+// One lane of a converged warp, the same one each time. The MMA warp runs its
+// loop as a whole and elects only for the instructions: their operands then
+// stay in uniform registers (with `if (lane == 0)` around the loop an MMA took
+// about 150 cycles to issue, longer than it takes to run).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+// NaN if any operand is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
                                             int c3) {
   asm volatile(
@@ -89,7 +160,8 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 // D (TMEM) (+)= A (TMEM) . B (shared memory descriptor)
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+          d),
       "r"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
@@ -143,15 +215,6 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32])
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// 16 columns, as above
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-          taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -169,38 +232,44 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __shared__ int abort_s, issued_s;
   volatile int* abort_flag = &abort_s;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + C::kStages + s); };
-  constexpr int kB = 2 * C::kStages;
+  // by value block (keys share the stages): the block's hidden rows are zeroed
+  auto fixed_bar = [&](int s) { return smem_u32(bars + 2 * C::kStages + s); };
+  constexpr int kB = 3 * C::kStages;
   const uint32_t q_full = smem_u32(bars + kB);
-  auto s_full = [&](int i) { return smem_u32(bars + kB + 1 + i); };
-  auto p_full = [&](int i) { return smem_u32(bars + kB + 3 + i); };
-  auto pv_done = [&](int i) { return smem_u32(bars + kB + 5 + i); };
-  const uint32_t drain_bar = smem_u32(bars + kB + 7);
-  auto fixed_bar = [&](int s) { return smem_u32(bars + kB + 8 + s); };
-  static_assert((kB + 8 + C::kStages) * 8 <= 512, "barriers");
+  auto s_full = [&](int i, int b) { return smem_u32(bars + kB + 1 + 2 * i + b); };  // scores of lane i, buffer b
+  auto p_full = [&](int i, int b) { return smem_u32(bars + kB + 5 + 2 * i + b); };
+  auto pv_done = [&](int i) { return smem_u32(bars + kB + 9 + i); };
+  auto drain_bar = [&](int i) { return smem_u32(bars + kB + 11 + i); };
+  static_assert((kB + 13) * 8 <= 512, "barriers");
 
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 32) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(empty_bar(s), 2);  // both lanes' MMAs
       mbar_init(fixed_bar(s), 1);
     }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), 4);
       mbar_init(pv_done(i), 1);
+      mbar_init(drain_bar(i), 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(s_full(i, b), 1);
+        mbar_init(p_full(i, b), 4);
+      }
     }
-    mbar_init(drain_bar, 1);
     abort_s = 0;
     issued_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&a.tmQ);
+    prefetch_map(&a.tmK);
+    prefetch_map(&a.tmV);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (!find_piece<kMT, kKB, kThreads>(a, blockIdx.x, scan, &g_paged_tc_status)) return;
+  if (!find_piece<kKB, kThreads, true>(a, blockIdx.x, scan, &g_paged_tc_status)) return;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
                  "n"(512)
@@ -213,234 +282,233 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const uint32_t tmem = tmem_holder;
 
   const Piece pc = scan.p;
-  const Seq sq = sequence(a, pc.b);
-  const int row0 = pc.tile * kMT, nrows = min(kMT, sq.tokens * a.group - row0);
-  const int tok0 = row0 / a.group, tok1 = (row0 + nrows - 1) / a.group;
+  const Seq sq = scan.seq;
+  const int row0 = pc.tile * a.tile_rows, nrows = min(a.tile_rows, sq.tokens * a.group - row0);
+  const int tok0 = row0 / a.group, tok1 = tok0 + (nrows - 1) / a.group;
   const Keys ks = tile_keys<kKB>(a, sq, tok0, tok1);
   const int all = ks.blocks();
   const int j0 = (int)((int64_t)all * pc.piece / pc.pieces);
   const int n = (int)((int64_t)all * (pc.piece + 1) / pc.pieces) - j0;  // blocks of this piece
-  const bool two = nrows > 128;
+  const bool two = nrows > a.lane_rows;
+  // Copies run in the order of their use: K_0 K_1 V_0 K_2 V_1 .. K_{n-1}
+  // V_{n-2} V_{n-1}; copy t goes to stage t % kStages.
+  auto copy_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
+  auto copy_v = [&](int j) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
+  auto phase = [&](int t) { return (uint32_t)((t / C::kStages) & 1); };
 
-  // Registers: 384 x 168 at launch; the softmax warps take 216 each, the
-  // others give up down to 56.
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
-      // ------------------------------------------------ copies: K_0 V_0 K_1 V_1 ..
-      const int box = min(a.l.page_size, kKB), boxes = kKB / box;  // 1 .. 8
-      const int per_batch = 32 / boxes;
-      const int* table = a.b.page_table + (int64_t)pc.b * a.b.ld_table;
-      auto load_entries = [&](int it0) {
-        const int it = it0 + lane / boxes;
-        if (it >= n) return -1;
-        const int kb = ks.block(j0 + it) * kKB + (lane % boxes) * box;
-        if (!(kb < ks.hi && (kb + box > ks.lo || kb < ks.sink_end))) return -1;
-        const int page = table[kb >> a.l.page_log2];
-        if (page < 0 || page >= a.l.num_pages) {
-          atomicExch(&g_paged_tc_status, IE_ERR_INVALID_ARG);
-          return a.l.num_pages;  // outside the tensor map: zeros
-        }
-        return page;
-      };
-      int entries = load_entries(0), next = load_entries(per_batch), batch = 0, issued = 0;
-      for (int t = 0; t < 2 * n; ++t) {
-        const int it = t >> 1, s = t % C::kStages;
-        if (it >= batch + per_batch) {
-          batch += per_batch;
-          entries = next;
-          next = load_entries(batch + per_batch);
-        }
-        if (!__all_sync(0xffffffffu, wait(empty_bar(s), (uint32_t)(((t / C::kStages) & 1) ^ 1), abort_flag))) break;
-        // lane x * (D / 64) + h copies half h of box x
-        const int x = lane / (D / 64), h = lane % (D / 64);
-        const int page = __shfl_sync(0xffffffffu, entries, (it - batch) * boxes + min(x, boxes - 1));
-        const bool mine = x < boxes && page >= 0;
-        const int copies = __popc(__ballot_sync(0xffffffffu, mine));
-        if (lane == 0) mbar_expect_tx(full_bar(s), copies * box * 128);
-        __syncwarp();
-        if (mine) {
-          const int kb = ks.block(j0 + it) * kKB + x * box, r = kb & (a.l.page_size - 1);
-          tma_load_4d(smem_u32(smem + C::kOffRing + s * C::kTile) + h * C::kHalf + x * box * 128,
-                      (t & 1) ? &a.tmV : &a.tmK, full_bar(s), 64 * h, a.swap_rc ? pc.head : r, a.swap_rc ? r : pc.head,
-                      page);
-        }
-        issued = t + 1;
+  if (warp == 0) {
+    // ------------------------------------------------ copies
+    const int box = min(a.l.page_size, kKB), boxes = kKB / box;  // rows of a copy, copies of a block's half
+    const int per_batch = 32 / boxes;                            // blocks whose table entries the warp holds
+    const int* table = a.b.page_table + (int64_t)pc.b * a.b.ld_table;
+    auto load_entries = [&](int it0) {
+      const int it = it0 + lane / boxes;
+      if (it >= n) return -1;
+      const int kb = ks.block(j0 + it) * kKB + (lane % boxes) * box;
+      if (!(kb < ks.hi && (kb + box > ks.lo || kb < ks.sink_end))) return -1;
+      const int page = table[kb >> a.l.page_log2];
+      if (page < 0 || page >= a.l.num_pages) {
+        atomicExch(&g_paged_tc_status, IE_ERR_INVALID_ARG);
+        return a.l.num_pages;  // outside the tensor map: zeros
       }
-      if (lane == 0) issued_s = issued;
-    } else if (warp == 1) {
-      if (lane == 0) {
-        // ---------------------------------------------- MMAs
-        const uint32_t id_qk = idesc_f16<T>(128, kKB, 0), id_pv = idesc_f16<T>(128, D, 1);
-        const uint32_t ring = smem_u32(smem + C::kOffRing);
-        bool any = false;
-        auto qk = [&](int i, int it) {  // S_i = Q_i K_it^T (copy 2 it)
-          if (it > 0 && !wait(pv_done(i), (uint32_t)((it - 1) & 1), abort_flag)) return false;
-          fence_after();
-          const uint32_t sk = ring + (uint32_t)((2 * it) % C::kStages) * C::kTile;
-          const uint32_t sq_ = smem_u32(smem) + i * C::kTile;
+      return page;
+    };
+    // lane x * (D / 64) + h copies half h of box x
+    const int x = lane / (D / 64), h = lane % (D / 64);
+    if (n > 0 && lane == 0) {
+      mbar_expect_tx(q_full, (two ? 2 : 1) * a.lane_rows * D * 2);
+      for (int i = 0; i < (two ? 2 : 1); ++i)
+#pragma unroll
+        for (int hh = 0; hh < D / 64; ++hh)
+          tma_load_3d(smem_u32(smem + i * C::kQTile + hh * C::kQHalf), &a.tmQ, q_full, 64 * hh, pc.head * a.group,
+                      sq.start + tok0 + i * (a.lane_rows / a.group));
+    }
+    // the entries a value block needs are at most two blocks behind the keys'
+    int entries[2] = {load_entries(0), load_entries(per_batch)}, batch = 0, issued = 0;
+    for (int t = 0; t < 2 * n; ++t) {
+      const bool is_v = t == 2 * n - 1 || (t > 0 && (t & 1) == 0);
+      const int it = t == 0 ? 0 : t == 2 * n - 1 ? n - 1 : is_v ? t / 2 - 1 : (t + 1) / 2, s = t % C::kStages;
+      if (it >= batch + 2 * per_batch) {  // keys ran past both batches: the older one's values are done
+        batch += per_batch;
+        entries[0] = entries[1];
+        entries[1] = load_entries(batch + per_batch);
+      }
+      if (!__all_sync(0xffffffffu, wait(empty_bar(s), phase(t) ^ 1u, abort_flag))) break;
+      const int at = it - batch, e = (at % per_batch) * boxes + min(x, boxes - 1);
+      const int p0 = __shfl_sync(0xffffffffu, entries[0], e), p1 = __shfl_sync(0xffffffffu, entries[1], e);
+      const int page = at < per_batch ? p0 : p1;
+      const bool mine = x < boxes && page >= 0;
+      const int copies = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) mbar_expect_tx(full_bar(s), copies * box * 128);
+      __syncwarp();
+      if (mine) {
+        const int r = (ks.block(j0 + it) * kKB + x * box) & (a.l.page_size - 1);
+        tma_load_4d(smem_u32(smem + C::kOffRing + s * C::kTile) + h * C::kHalf + x * box * 128,
+                    is_v ? &a.tmV : &a.tmK, full_bar(s), 64 * h, a.swap_rc ? pc.head : r, a.swap_rc ? r : pc.head,
+                    page);
+      }
+      issued = t + 1;
+    }
+    if (lane == 0) issued_s = issued;
+  } else if (warp == 1 || warp == 3) {
+    const int i = warp >> 1;
+    if (n > 0 && (i == 0 || two)) {
+      // ---------------------------------------------- MMAs of lane i
+      const uint32_t id_qk = idesc_f16<T>(128, kKB, 0), id_pv = idesc_f16<T>(128, D, 1);
+      const uint32_t ring = smem_u32(smem + C::kOffRing);
+      const uint64_t qs = sw128_desc(smem_u32(smem) + i * C::kQTile);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + 128 * i;
+      const int nu = __shfl_sync(0xffffffffu, n, 0);
+      const bool alone = __shfl_sync(0xffffffffu, (int)two, 0) == 0;
+      auto over = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait(bar, parity, abort_flag)) != 0;
+      };
+      // the stage is free when both lanes' MMAs so far are done
+      auto release = [&](int t) {
+        mma_commit(empty_bar(t % C::kStages));
+        if (alone) mma_commit(empty_bar(t % C::kStages));
+      };
+      auto qk = [&](int j) {  // scores of block j
+        const int t = copy_k(j);
+        if (!over(full_bar(t % C::kStages), phase(t))) return false;
+        fence_after();
+        const uint64_t sk = sw128_desc(ring + (uint32_t)(t % C::kStages) * C::kTile);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_f16(tmem + 128 * i, sw128_desc(sq_ + (uint32_t)(k >> 2) * C::kHalf) + 2 * (k & 3),
-                    sw128_desc(sk + (uint32_t)(k >> 2) * C::kHalf) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
-          mma_commit(s_full(i));
-          any = true;
-          return true;
-        };
-        auto pv = [&](int i, int it) {  // O_i += P_i V_it (copy 2 it + 1)
-          if (!wait(p_full(i), (uint32_t)(it & 1), abort_flag)) return false;
-          fence_after();
-          const uint32_t sv = ring + (uint32_t)((2 * it + 1) % C::kStages) * C::kTile;
+            mma_f16(tm + 64 * (j & 1), qs + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
+                    sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
+          mma_commit(s_full(i, j & 1));
+          release(t);
+        }
+        return true;
+      };
+      bool ok = over(q_full, 0);
+      for (int j = 0; ok && j < min(nu, 2); ++j) ok = qk(j);
+      for (int j = 0; ok && j < nu; ++j) {
+        const int t = copy_v(j);
+        ok = over(fixed_bar(j % C::kStages), (uint32_t)((j / C::kStages) & 1)) &&
+             over(p_full(i, j & 1), (uint32_t)((j >> 1) & 1));
+        if (!ok) break;
+        fence_after();
+        const uint64_t sv = sw128_desc_mn(ring + (uint32_t)(t % C::kStages) * C::kTile, C::kHalf);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kKB / 16; ++k)
-            mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, sw128_desc_mn(sv + (uint32_t)k * 16 * 128, C::kHalf),
-                   id_pv, (it | k) != 0 ? 1u : 0u);
+            mma_ts(tm + 256, tm + 64 * (j & 1) + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
           mma_commit(pv_done(i));
-          any = true;
-          return true;
-        };
-        auto arrived = [&](int t) {
-          return wait(full_bar(t % C::kStages), (uint32_t)((t / C::kStages) & 1), abort_flag);
-        };
-        auto release = [&](int t) { mma_commit(empty_bar(t % C::kStages)); };
-        bool ok = wait(q_full, 0, abort_flag);
-        fence_after();
-        if (ok && n > 0) {
-          ok = arrived(0) && qk(0, 0) && (!two || qk(1, 0));
-          if (ok) release(0);
-          for (int it = 0; ok && it < n; ++it) {
-            // P_0 V_it, S_0 of the next block, P_1 V_it, S_1 of the next block
-            ok = arrived(2 * it + 1) && wait(fixed_bar(it % C::kStages), (uint32_t)((it / C::kStages) & 1), abort_flag);
-            const bool more = it + 1 < n;
-            ok = ok && pv(0, it);
-            if (!two && ok) release(2 * it + 1);
-            if (ok && more) ok = arrived(2 * it + 2) && qk(0, it + 1);
-            if (!two && ok && more) release(2 * it + 2);
-            if (two) {
-              ok = ok && pv(1, it);
-              if (ok) release(2 * it + 1);
-              if (ok && more) ok = qk(1, it + 1);
-              if (ok && more) release(2 * it + 2);
-            }
-          }
+          release(t);
         }
-        if (*abort_flag && any) {
-          mma_commit(drain_bar);
-          const unsigned long long t0 = globaltimer();
-          while (!mbar_try(drain_bar, 0) && globaltimer() - t0 < kDrainWaitNs) {
-          }
+        // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
+        if (j + 2 < nu) ok = over(pv_done(i), (uint32_t)(j & 1)) && qk(j + 2);
+      }
+      if (*abort_flag) {
+        // every MMA issued so far is done before TMEM is released
+        __syncwarp();
+        if (elect_one()) mma_commit(drain_bar(i));
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try(drain_bar(i), 0) && globaltimer() - t0 < kDrainWaitNs) {
         }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------ value rows nobody sees
+    // (it passes every value block on, so that it never falls a ring behind)
+    for (int j = 0; j < n; ++j) {
+      const int kb = ks.block(j0 + j) * kKB, t = copy_v(j), s = t % C::kStages;
+      if (!__all_sync(0xffffffffu, wait(full_bar(s), phase(t), abort_flag))) break;
+      if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
+        uint8_t* v = smem + C::kOffRing + s * C::kTile;
+        for (int r = lane; r < kKB; r += 32) {
+          const int key = kb + r;
+          if (!(key < ks.hi && (key >= ks.lo || key < ks.sink_end)))
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
-    } else if (warp == 2) {
-      // ------------------------------------------------ value rows nobody sees
-      // (it passes every value block on, so that it never falls a ring behind)
-      for (int it = 0; it < n; ++it) {
-        const int kb = ks.block(j0 + it) * kKB;
-        const int t = 2 * it + 1, s = t % C::kStages;
-        if (!__all_sync(0xffffffffu, wait(full_bar(s), (uint32_t)((t / C::kStages) & 1), abort_flag))) break;
-        if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
-          uint8_t* v = smem + C::kOffRing + s * C::kTile;
-          for (int r = lane; r < kKB; r += 32) {
-            const int j = kb + r;
-            if (!(j < ks.hi && (j >= ks.lo || j < ks.sink_end)))
-#pragma unroll
-              for (int c = 0; c < D / 8; ++c)
-                *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(fixed_bar(it % C::kStages));  // by value block: keys use the stages too
-      }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      if (lane == 0) mbar_arrive(fixed_bar(j % C::kStages));
+    }
+  } else if (warp >= 4) {
     // ------------------------------------------------ softmax and epilogue
     const int i = (warp - 4) >> 2, quad = warp & 3;  // TMEM lane quarter = warp & 3
-    const int r = 32 * quad + lane, row = 128 * i + r;
+    const int r = 32 * quad + lane;                  // row of the lane
+    const int row = r < a.lane_rows ? i * a.lane_rows + r : INT_MAX;  // row of the tile
     const uint32_t tl = (uint32_t)(32 * quad) << 16;
-    const uint32_t ts = tmem + tl + 128 * i, to = tmem + tl + 256 + 128 * i;
-    {
-      // this warp's 32 rows of Q, D / 8 lanes a row
-      constexpr int kChunks = D / 8, kRows = 32 / kChunks;
-      uint8_t* qs = smem + i * C::kTile;
-#pragma unroll 4
-      for (int x = 0; x < 32 / kRows; ++x) {
-        const int rr = 32 * quad + x * kRows + lane / kChunks, c = lane % kChunks, g = row0 + 128 * i + rr;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (128 * i + rr < nrows)
-          w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(sq.start + g / a.group) * a.ldq +
-                                              (int64_t)(pc.head * a.group + g % a.group) * a.hsq + 8 * c);
-        *reinterpret_cast<uint4*>(qs + (c >> 3) * C::kHalf + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
-    const int tok = (row0 + row) / a.group;
-    const int pos = row < nrows ? sq.pos0 + tok : -1;
-    const int pos_min = sq.pos0 + (row0 + 128 * i) / a.group;
-    const int pos_max = sq.pos0 + (row0 + min(nrows, 128 * i + 128) - 1) / a.group;
+    const uint32_t to = tmem + tl + 256 + 128 * i;
+    const int last = min(nrows, (i + 1) * a.lane_rows) - 1;  // the lane's last row
+    const int pos = row < nrows ? sq.pos0 + tok0 + row / a.group : -1;
+    const int pos_min = sq.pos0 + tok0 + i * a.lane_rows / a.group, pos_max = sq.pos0 + tok0 + last / a.group;
     // a scale of 0 weighs all seen keys alike: scores 0, so that masked ones can stay infinite
     const bool flat = a.scale_log2 == 0.f;
     const float c = flat ? 1.0f : a.scale_log2;
-    const float hidden = c > 0.f ? -INFINITY : INFINITY;
     float m = -INFINITY, l = 0.f;  // m: the reference, in log2 units
     bool ok = true;
     if (i == 0 || two) {
-      for (int it = 0; it < n; ++it) {
-        const int kb = ks.block(j0 + it) * kKB;
-        if (!wait(s_full(i), (uint32_t)(it & 1), abort_flag)) { ok = false; break; }
+      for (int j = 0; j < n; ++j) {
+        const int kb = ks.block(j0 + j) * kKB;
+        const uint32_t ts = tmem + tl + 128 * i + 64 * (j & 1);
+        ok = __all_sync(0xffffffffu, wait(s_full(i, j & 1), (uint32_t)((j >> 1) & 1), abort_flag));
+        if (!ok) break;
         fence_after();
-        float v[128];
+        float v[kKB];
         {
-          uint32_t r0[64], r1[64];
-          tmem_ld(ts, r0);
-          tmem_ld(ts + 64, r1);
-          tmem_ld_wait(r0);
-          tmem_ld_wait(r1);
+          uint32_t w[kKB];
+          tmem_ld(ts, w);
+          tmem_ld_wait(w);
 #pragma unroll
-          for (int x = 0; x < 64; ++x) {
-            v[x] = __uint_as_float(r0[x]);
-            v[64 + x] = __uint_as_float(r1[x]);
-          }
+          for (int x = 0; x < kKB; ++x) v[x] = __uint_as_float(w[x]);
         }
+        const bool masked = kb + kKB - 1 > pos_min || (a.window && (int64_t)pos_max - kb >= a.window);
         if (flat) {
 #pragma unroll
-          for (int x = 0; x < 128; ++x) v[x] = 0.f;
+          for (int x = 0; x < kKB; ++x) v[x] = 0.f;
         }
-        if (kb + kKB - 1 > pos_min || (a.window && (int64_t)pos_max - kb >= a.window)) {
+        if (masked) {
+          const float hidden = c > 0.f ? -INFINITY : INFINITY;
           const int hi = pos - kb;  // columns <= hi
           if (!a.window) {
 #pragma unroll
-            for (int x = 0; x < 128; ++x) v[x] = x <= hi ? v[x] : hidden;
+            for (int x = 0; x < kKB; ++x) v[x] = x <= hi ? v[x] : hidden;
           } else {
             const int64_t lo64 = (int64_t)pos - a.window - kb;
             const int lo = (int)(lo64 < -1 ? -1 : lo64), sk = a.sinks - kb;  // columns > lo or < sk
 #pragma unroll
-            for (int x = 0; x < 128; ++x)
-              v[x] = x <= hi && (x > lo || x < sk) ? v[x] : hidden;
+            for (int x = 0; x < kKB; ++x) v[x] = x <= hi && (x > lo || x < sk) ? v[x] : hidden;
           }
         }
         // the row's largest scaled score
-        float t[4] = {v[0], v[1], v[2], v[3]};
-        if (c > 0.f) {
+        float top;
+        {
+          if (c > 0.f) {
+            float t[4];
 #pragma unroll
-          for (int x = 4; x < 128; ++x) t[x & 3] = fmaxf(t[x & 3], v[x]);
-          t[0] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-        } else {
+            for (int x = 0; x < 4; ++x) t[x] = v[x];
 #pragma unroll
-          for (int x = 4; x < 128; ++x) t[x & 3] = fminf(t[x & 3], v[x]);
-          t[0] = fminf(fminf(t[0], t[1]), fminf(t[2], t[3]));
+            for (int x = 4; x + 8 <= kKB; x += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) t[y] = max3(t[y], v[x + 2 * y], v[x + 2 * y + 1]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) t[y] = max3(t[y], v[kKB - 4 + 2 * y], v[kKB - 3 + 2 * y]);
+            top = max3(max3(t[0], t[1], t[2]), t[3], t[3]) * c;
+          } else {
+            top = v[0] * c;
+#pragma unroll
+            for (int x = 1; x < kKB; ++x) top = max3(top, v[x] * c, top);
+          }
         }
-        const float top = t[0] * c;
-        const bool rise = top > m + kLazy;
+        // (a NaN or infinite score turns the row's reference, and with it the row, into NaN)
+        const bool rise = row < nrows && !(top <= m + kLazy);
         if (__any_sync(0xffffffffu, rise)) {
-          const float to_m = rise ? top : m;
+          const float to_m = !rise ? m : top < INFINITY ? top : __int_as_float(0x7fffffff);
           const float f = rise ? ex2(m - to_m) : 1.0f;
-          if (it > 0) {
-            if (!wait(pv_done(i), (uint32_t)((it - 1) & 1), abort_flag)) { ok = false; break; }
+          if (j > 0) {
+            // every product before this block's
+            ok = __all_sync(0xffffffffu, wait(pv_done(i), (uint32_t)((j - 1) & 1), abort_flag));
+            if (!ok) break;
             fence_after();
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
@@ -456,77 +524,108 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           m = to_m;
         }
         const float mb = m == -INFINITY ? 0.f : -m;
-        float l0 = 0.f, l1 = 0.f;
+        const uint64_t c2 = pair(c, c), mb2 = pair(mb, mb);
+        uint64_t l2 = pair(0.f, 0.f);
+        uint32_t pk[kKB / 2];
+        // the polynomial has no 0 for a masked score: such blocks do without
+        auto exps = [&](auto poly) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            const float e0 = ex2(fmaf(v[32 * x + 2 * y], c, mb)), e1 = ex2(fmaf(v[32 * x + 2 * y + 1], c, mb));
-            l0 += e0;
-            l1 += e1;
+          for (int y = 0; y < kKB / 2; ++y) {
+            float e0, e1;
+            split(fma2(pair(v[2 * y], v[2 * y + 1]), c2, mb2), e0, e1);
+            if (y % 8 < decltype(poly)::value) {
+              ex2_poly2(e0, e1);
+            } else {
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+            }
+            l2 = add2(l2, pair(e0, e1));
             pk[y] = pack2<T>(e0, e1);
           }
-          tmem_st(ts + 16 * x, pk);
+        };
+        if (masked) exps(std::integral_constant<int, 0>{});
+        else exps(std::integral_constant<int, C::kPoly>{});
+        tmem_st(ts, pk);
+        {
+          float l0, l1;
+          split(l2, l0, l1);
+          l += l0 + l1;
         }
-        l += l0 + l1;
         tmem_st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(i));
+        if (lane == 0) mbar_arrive(p_full(i, j & 1));
       }
     }
-    // ---- epilogue: one row a thread
+    // ---- epilogue
     const bool cut = pc.slot >= 0;
-    if (ok && n > 0 && (i == 0 || two)) ok = wait(pv_done(i), (uint32_t)((n - 1) & 1), abort_flag);
-    if (ok && !*abort_flag && 128 * i < nrows && (!cut || (pc.slot < a.slot_cap && pc.split < a.split_cap))) {
+    if (i == 0 || two) {
+      // in order: the scores of the last block only say that the product three before the end is done
+      if (ok && n > 1) ok = wait(pv_done(i), (uint32_t)((n - 2) & 1), abort_flag);
+      if (ok && n > 0) ok = wait(pv_done(i), (uint32_t)((n - 1) & 1), abort_flag);
+      ok = __all_sync(0xffffffffu, ok) && (!cut || (pc.slot < a.slot_cap && pc.split < a.split_cap));
       fence_after();
-      const float inv = l > 0.f ? 1.0f / l : 0.f;
-      const int g = row0 + row;
-      T* dst = static_cast<T*>(a.out) + (int64_t)(sq.start + g / a.group) * a.ld_out +
-               (int64_t)(pc.head * a.group + g % a.group) * D;
-      float* po = a.part_o + ((int64_t)pc.slot * kMT + row) * D;
+      if (ok && cut) {
+        // row-interleaved 16-byte pieces, so that a warp's stores are contiguous
+        float4* po = reinterpret_cast<float4*>(a.part_o) + ((int64_t)pc.slot * 8 + 4 * i + quad) * (D / 4) * 32 + lane;
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) {
-        float o[32];
-        if (n > 0) {
-          uint32_t w[32];
-          tmem_ld(to + 32 * x, w);
-          tmem_ld_wait(w);
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t w[32] = {};
+          if (n > 0) {
+            tmem_ld(to + 32 * x, w);
+            tmem_ld_wait(w);
+          }
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = __uint_as_float(w[y]);
-        } else {
-#pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = 0.f;
+          for (int y = 0; y < 8; ++y)
+            po[(8 * x + y) * 32] = make_float4(__uint_as_float(w[4 * y]), __uint_as_float(w[4 * y + 1]),
+                                               __uint_as_float(w[4 * y + 2]), __uint_as_float(w[4 * y + 3]));
         }
-        if (row < nrows) {
-          if (cut) {
+        a.part_ml[(int64_t)pc.slot * kRowsChunk + 128 * i + r] = make_float2(m, l);
+        if (pc.piece == 0 && i == 0 && r == 0) {
+          Split sp = {};
+          sp.slot0 = pc.slot;
+          sp.pieces = pc.pieces;
+          sp.token0 = sq.start + tok0;
+          sp.rows = nrows;
+          sp.head0 = pc.head * a.group;
+          a.splits[pc.split] = sp;
+        }
+      } else if (ok) {
+        // through the lane's Q tile (its products are done): swizzled rows in,
+        // D / 8 lanes a row out
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        uint8_t* st = smem + i * C::kQTile + 32 * quad * D * 2;
 #pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              *reinterpret_cast<float4*>(po + 32 * x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-          } else {
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t w[32] = {};
+          if (n > 0) {
+            tmem_ld(to + 32 * x, w);
+            tmem_ld_wait(w);
+          }
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              uint4 w;
-              w.x = pack2<T>(o[y] * inv, o[y + 1] * inv);
-              w.y = pack2<T>(o[y + 2] * inv, o[y + 3] * inv);
-              w.z = pack2<T>(o[y + 4] * inv, o[y + 5] * inv);
-              w.w = pack2<T>(o[y + 6] * inv, o[y + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + 32 * x + y) = w;
-            }
+          for (int y = 0; y < 4; ++y) {
+            uint4 u;
+            u.x = pack2<T>(__uint_as_float(w[8 * y]) * inv, __uint_as_float(w[8 * y + 1]) * inv);
+            u.y = pack2<T>(__uint_as_float(w[8 * y + 2]) * inv, __uint_as_float(w[8 * y + 3]) * inv);
+            u.z = pack2<T>(__uint_as_float(w[8 * y + 4]) * inv, __uint_as_float(w[8 * y + 5]) * inv);
+            u.w = pack2<T>(__uint_as_float(w[8 * y + 6]) * inv, __uint_as_float(w[8 * y + 7]) * inv);
+            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * x + y) ^ (lane & 7)) << 4)) = u;
           }
         }
-      }
-      if (cut && row < nrows) a.part_ml[(int64_t)pc.slot * kMT + row] = make_float2(m, l);
-      if (cut && pc.piece == 0 && row == 0) {
-        Split s = {};
-        s.slot0 = pc.slot;
-        s.pieces = pc.pieces;
-        s.token0 = sq.start;
-        s.rows = nrows;
-        s.head0 = pc.head * a.group;
-        s.row0 = row0;
-        a.splits[pc.split] = s;
+        __syncwarp();
+        constexpr int kChunks = D / 8, kRows = 32 / kChunks;
+        const int cc = lane % kChunks;
+        T* out = static_cast<T*>(a.out) + (int64_t)(sq.start + tok0) * a.ld_out + (int64_t)pc.head * a.group * D +
+                 8 * cc;
+#pragma unroll 4
+        for (int x = 0; x < 32 / kRows; ++x) {
+          const int q = x * kRows + lane / kChunks, rr = 32 * quad + q, g = i * a.lane_rows + rr;
+          if (rr < a.lane_rows && g < nrows) {
+            const int tok = g / a.group;
+            *reinterpret_cast<uint4*>(out + (int64_t)tok * a.ld_out + (g - tok * a.group) * D) =
+                *reinterpret_cast<const uint4*>(st + q * D * 2 + ((cc ^ (q & 7)) << 4));
+          }
+        }
       }
     }
   }
@@ -536,10 +635,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __syncthreads();
   fence_after();
   if (*abort_flag && threadIdx.x == 0) {
-    // copies still in flight land before the CTA exits: the last kStages
-    for (int t = max(0, issued_s - C::kStages); t < issued_s; ++t) {
+    // copies still in flight land before the CTA exits: the queries and the last kStages
+    for (int t = max(0, issued_s - C::kStages) - 1; t < issued_s; ++t) {
+      const bool queries = t < max(0, issued_s - C::kStages);
       const unsigned long long t0 = globaltimer();
-      while (!mbar_try(full_bar(t % C::kStages), (uint32_t)((t / C::kStages) & 1)) &&
+      while (!mbar_try(queries ? q_full : full_bar(t % C::kStages), queries ? 0u : phase(t)) &&
              globaltimer() - t0 < kDrainWaitNs / 4) {
       }
     }
@@ -548,8 +648,65 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
+// Joins the cut tiles' pieces in piece order, 32 rows (one warp's of the chunk
+// kernel) a CTA: a thread has one row, its warp every fourth 16-byte piece of
+// the row's outputs, as the chunk kernel stored them. The rows go out through
+// shared memory.
 template <typename T, int D>
-int launch(Args& a, int64_t grid, cudaStream_t st) {
+__global__ void __launch_bounds__(128) join_chunks_kernel(const __grid_constant__ Args a) {
+  constexpr int kMine = D / 16, kPitch = D * 2 + 8;
+  __shared__ __align__(16) uint8_t rows_s[32 * kPitch];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nkv = a.l.n_kv_heads;
+  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * 8;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const Split sp = a.splits[it >> 3];
+    const int part = (int)(it & 7), i = part >> 2, r0 = 32 * (part & 3);  // lane of the tile, first row there
+    if (r0 >= a.lane_rows || i * a.lane_rows + r0 >= sp.rows) continue;   // the same for the whole block
+    float top = -INFINITY;
+    for (int s = 0; s < sp.pieces; ++s)
+      top = fmaxf(top, a.part_ml[((int64_t)sp.slot0 + (int64_t)s * nkv) * kRowsChunk + 32 * part + lane].x);
+    float4 acc[kMine];
+#pragma unroll
+    for (int x = 0; x < kMine; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 2
+    for (int s = 0; s < sp.pieces; ++s) {
+      const int64_t slot = (int64_t)sp.slot0 + (int64_t)s * nkv;
+      const float2 ml = a.part_ml[slot * kRowsChunk + 32 * part + lane];
+      const float f = top == -INFINITY ? 0.f : ex2(ml.x - top);
+      sum += f * ml.y;
+      const float4* po = reinterpret_cast<const float4*>(a.part_o) + (slot * 8 + part) * (D / 4) * 32 + lane;
+#pragma unroll
+      for (int x = 0; x < kMine; ++x) {
+        const float4 u = po[(warp + 4 * x) * 32];
+        acc[x].x += f * u.x;
+        acc[x].y += f * u.y;
+        acc[x].z += f * u.z;
+        acc[x].w += f * u.w;
+      }
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+    for (int x = 0; x < kMine; ++x)
+      *reinterpret_cast<uint2*>(rows_s + lane * kPitch + (warp + 4 * x) * 8) =
+          make_uint2(pack2<T>(acc[x].x * inv, acc[x].y * inv), pack2<T>(acc[x].z * inv, acc[x].w * inv));
+    __syncthreads();
+    constexpr int kLanes = D / 4, kRows = 128 / kLanes;  // 8 bytes a thread
+    for (int q = threadIdx.x / kLanes; q < 32; q += kRows) {
+      const int cc = threadIdx.x % kLanes, g = i * a.lane_rows + r0 + q;
+      if (r0 + q < a.lane_rows && g < sp.rows)
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(sp.token0 + g / a.group) * a.ld_out +
+                                  (int64_t)(sp.head0 + g % a.group) * D + 4 * cc) =
+            *reinterpret_cast<const uint2*>(rows_s + q * kPitch + cc * 8);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int D>
+int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
   auto kernel = chunk_kernel<T, D>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return IE_ERR_LAUNCH;
@@ -559,8 +716,23 @@ int launch(Args& a, int64_t grid, cudaStream_t st) {
       return IE_ERR_LAUNCH;
     configured[dev] = true;
   }
+  const int64_t grid = most_tiles + a.slot_cap;
+  if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
   kernel<<<(unsigned)grid, kThreads, Cfg<D>::kSmem, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) {
+    const int64_t items = 8 * (most_tiles < a.target ? most_tiles : a.target);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items < 148 * 8 ? items : 148 * 8));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_launch_enabled() ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, join_chunks_kernel<T, D>, a);
+  }
   if (e != cudaSuccess) {
     std::fprintf(stderr, "infengine_b200: paged attention launch failed: %s\n", cudaGetErrorString(e));
     return IE_ERR_LAUNCH;
@@ -570,9 +742,10 @@ int launch(Args& a, int64_t grid, cudaStream_t st) {
 
 }  // namespace
 
-int launch_chunks(ie_dtype dt, int D, Args& a, int64_t grid, cudaStream_t st) {
-  if (dt == IE_DTYPE_F16) return D == 128 ? launch<__half, 128>(a, grid, st) : launch<__half, 64>(a, grid, st);
-  return D == 128 ? launch<__nv_bfloat16, 128>(a, grid, st) : launch<__nv_bfloat16, 64>(a, grid, st);
+int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, cudaStream_t st) {
+  if (dt == IE_DTYPE_F16)
+    return D == 128 ? launch<__half, 128>(a, most_tiles, st) : launch<__half, 64>(a, most_tiles, st);
+  return D == 128 ? launch<__nv_bfloat16, 128>(a, most_tiles, st) : launch<__nv_bfloat16, 64>(a, most_tiles, st);
 }
 
 }  // namespace pa
