@@ -30,12 +30,14 @@
 // Operands are 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K
 // K-major, V MN-major as it arrives.
 //
-// Warp roles: 0 copies (Q, then TMA boxes of up to 64 rows of one page; the
-// lanes hold the next table entries), 1 and 3 issue the two lanes' MMAs (a
-// barrier wait costs an issuing warp about 110 cycles even when it is over,
-// and one warp for both lanes spent 2600 cycles a step on them), 2 zeroes value
-// rows that no row of the tile sees (range edges inside a block; what the page
-// holds there may be NaN), 4-7 and 8-11 the lanes' softmax and epilogue. Every
+// Warp roles: 0 copies queries and keys, 2 values (TMA boxes of up to 64 rows
+// of one page; the lanes hold the next table entries), 1 and 3 issue the two
+// lanes' MMAs, 4-7 and 8-11 are the lanes' softmax and epilogue. A barrier wait
+// costs an issuing warp about 110 cycles even when it is over, a TMA or MMA
+// some tens: with one warp for all copies a step of 64 keys took 1900 cycles
+// (2700 with pages of 16), with one for all MMAs 2600. Value rows that no row
+// of the tile sees (range edges inside a block; what the page holds there may
+// be NaN) are zeroed by the MMA warps before the product. Every
 // mbarrier wait is bounded: on expiry IE_ERR_TIMEOUT is recorded, all roles
 // leave their loops, and MMAs and copies in flight are waited for before TMEM
 // is freed.
@@ -229,31 +231,30 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
   __shared__ Scan scan;
   __shared__ uint32_t tmem_holder;
-  __shared__ int abort_s, issued_s;
+  __shared__ int abort_s, issued_s[2];
   volatile int* abort_flag = &abort_s;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + C::kStages + s); };
-  // by value block (keys share the stages): the block's hidden rows are zeroed
-  auto fixed_bar = [&](int s) { return smem_u32(bars + 2 * C::kStages + s); };
-  constexpr int kB = 3 * C::kStages;
+  constexpr int kB = 2 * C::kStages;
   const uint32_t q_full = smem_u32(bars + kB);
   auto s_full = [&](int i, int b) { return smem_u32(bars + kB + 1 + 2 * i + b); };  // scores of lane i, buffer b
   auto p_full = [&](int i, int b) { return smem_u32(bars + kB + 5 + 2 * i + b); };
   auto pv_done = [&](int i) { return smem_u32(bars + kB + 9 + i); };
-  auto drain_bar = [&](int i) { return smem_u32(bars + kB + 11 + i); };
-  static_assert((kB + 13) * 8 <= 512, "barriers");
+  auto o_full = [&](int i) { return smem_u32(bars + kB + 11 + i); };
+  auto drain_bar = [&](int i) { return smem_u32(bars + kB + 13 + i); };
+  static_assert((kB + 15) * 8 <= 512, "barriers");
 
   if (threadIdx.x == 32) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 2);  // both lanes' MMAs
-      mbar_init(fixed_bar(s), 1);
     }
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(pv_done(i), 1);
+      mbar_init(o_full(i), 1);
       mbar_init(drain_bar(i), 1);
       for (int b = 0; b < 2; ++b) {
         mbar_init(s_full(i, b), 1);
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
     }
     abort_s = 0;
-    issued_s = 0;
+    issued_s[0] = issued_s[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&a.tmQ);
     prefetch_map(&a.tmK);
@@ -290,21 +291,32 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const int j0 = (int)((int64_t)all * pc.piece / pc.pieces);
   const int n = (int)((int64_t)all * (pc.piece + 1) / pc.pieces) - j0;  // blocks of this piece
   const bool two = nrows > a.lane_rows;
-  // Copies run in the order of their use: K_0 K_1 V_0 K_2 V_1 .. K_{n-1}
-  // V_{n-2} V_{n-1}; copy t goes to stage t % kStages.
-  auto copy_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
-  auto copy_v = [&](int j) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
-  auto phase = [&](int t) { return (uint32_t)((t / C::kStages) & 1); };
+  // stage and phase of block j's keys (v = 0) or values (1): each has half the ring
+  constexpr int kDepth = C::kStages / 2;
+  auto stage = [&](int v, int j) { return v * kDepth + j % kDepth; };
+  auto phase = [&](int j) { return (uint32_t)((j / kDepth) & 1); };
 
-  if (warp == 0) {
-    // ------------------------------------------------ copies
-    const int box = min(a.l.page_size, kKB), boxes = kKB / box;  // rows of a copy, copies of a block's half
-    const int per_batch = 32 / boxes;                            // blocks whose table entries the warp holds
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------ copies of keys (0) or values (2)
+    const int v = warp >> 1;
+    const int nu = __shfl_sync(0xffffffffu, n, 0), head = __shfl_sync(0xffffffffu, pc.head, 0);
+    const CUtensorMap* map = v ? &a.tmV : &a.tmK;
+    if (v == 0 && nu > 0 && elect_one()) {
+      mbar_expect_tx(q_full, (two ? 2 : 1) * a.lane_rows * D * 2);
+      for (int i = 0; i < (two ? 2 : 1); ++i)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_3d(smem_u32(smem + i * C::kQTile + h * C::kQHalf), &a.tmQ, q_full, 64 * h, head * a.group,
+                      sq.start + tok0 + i * (a.lane_rows / a.group));
+    }
+    // rows of a copy, copies of a block's half, blocks whose table entries the warp holds
+    const int box_log2 = min(a.l.page_log2, 6), box = 1 << box_log2, boxes_log2 = 6 - box_log2;
+    const int held_log2 = 5 - boxes_log2;
     const int* table = a.b.page_table + (int64_t)pc.b * a.b.ld_table;
     auto load_entries = [&](int it0) {
-      const int it = it0 + lane / boxes;
+      const int it = it0 + (lane >> boxes_log2);
       if (it >= n) return -1;
-      const int kb = ks.block(j0 + it) * kKB + (lane % boxes) * box;
+      const int kb = ks.block(j0 + it) * kKB + (lane & ((1 << boxes_log2) - 1)) * box;
       if (!(kb < ks.hi && (kb + box > ks.lo || kb < ks.sink_end))) return -1;
       const int page = table[kb >> a.l.page_log2];
       if (page < 0 || page >= a.l.num_pages) {
@@ -313,43 +325,38 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
       return page;
     };
-    // lane x * (D / 64) + h copies half h of box x
-    const int x = lane / (D / 64), h = lane % (D / 64);
-    if (n > 0 && lane == 0) {
-      mbar_expect_tx(q_full, (two ? 2 : 1) * a.lane_rows * D * 2);
-      for (int i = 0; i < (two ? 2 : 1); ++i)
+    int entries = load_entries(0), next = load_entries(1 << held_log2), issued = 0;
+    for (int j = 0; j < nu; ++j) {
+      const int at = j & ((1 << held_log2) - 1);
+      if (j > 0 && at == 0) {
+        entries = next;
+        next = load_entries(j + (1 << held_log2));
+      }
+      const uint32_t full = full_bar(stage(v, j)), dst = smem_u32(smem + C::kOffRing + stage(v, j) * C::kTile);
+      const int r0 = (ks.block(j0 + j) * kKB) & (a.l.page_size - 1);
+      int page[4], copies = 0;
 #pragma unroll
-        for (int hh = 0; hh < D / 64; ++hh)
-          tma_load_3d(smem_u32(smem + i * C::kQTile + hh * C::kQHalf), &a.tmQ, q_full, 64 * hh, pc.head * a.group,
-                      sq.start + tok0 + i * (a.lane_rows / a.group));
-    }
-    // the entries a value block needs are at most two blocks behind the keys'
-    int entries[2] = {load_entries(0), load_entries(per_batch)}, batch = 0, issued = 0;
-    for (int t = 0; t < 2 * n; ++t) {
-      const bool is_v = t == 2 * n - 1 || (t > 0 && (t & 1) == 0);
-      const int it = t == 0 ? 0 : t == 2 * n - 1 ? n - 1 : is_v ? t / 2 - 1 : (t + 1) / 2, s = t % C::kStages;
-      if (it >= batch + 2 * per_batch) {  // keys ran past both batches: the older one's values are done
-        batch += per_batch;
-        entries[0] = entries[1];
-        entries[1] = load_entries(batch + per_batch);
+      for (int x = 0; x < 4; ++x) {
+        page[x] = __shfl_sync(0xffffffffu, entries, ((at << boxes_log2) + x) & 31);
+        if (x >> boxes_log2) page[x] = -1;
+        copies += page[x] >= 0;
       }
-      if (!__all_sync(0xffffffffu, wait(empty_bar(s), phase(t) ^ 1u, abort_flag))) break;
-      const int at = it - batch, e = (at % per_batch) * boxes + min(x, boxes - 1);
-      const int p0 = __shfl_sync(0xffffffffu, entries[0], e), p1 = __shfl_sync(0xffffffffu, entries[1], e);
-      const int page = at < per_batch ? p0 : p1;
-      const bool mine = x < boxes && page >= 0;
-      const int copies = __popc(__ballot_sync(0xffffffffu, mine));
-      if (lane == 0) mbar_expect_tx(full_bar(s), copies * box * 128);
-      __syncwarp();
-      if (mine) {
-        const int r = (ks.block(j0 + it) * kKB + x * box) & (a.l.page_size - 1);
-        tma_load_4d(smem_u32(smem + C::kOffRing + s * C::kTile) + h * C::kHalf + x * box * 128,
-                    is_v ? &a.tmV : &a.tmK, full_bar(s), 64 * h, a.swap_rc ? pc.head : r, a.swap_rc ? r : pc.head,
-                    page);
+      if (!__all_sync(0xffffffffu, wait(empty_bar(stage(v, j)), phase(j) ^ 1u, abort_flag))) break;
+      if (elect_one()) {
+        mbar_expect_tx(full, copies * box * D * 2);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (page[x] >= 0) {
+            const int r = (r0 + x * box) & (a.l.page_size - 1);
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              tma_load_4d(dst + h * C::kHalf + x * box * 128, map, full, 64 * h, a.swap_rc ? head : r,
+                          a.swap_rc ? r : head, page[x]);
+          }
       }
-      issued = t + 1;
+      issued = j + 1;
     }
-    if (lane == 0) issued_s = issued;
+    if (lane == 0) issued_s[v] = issued;
   } else if (warp == 1 || warp == 3) {
     const int i = warp >> 1;
     if (n > 0 && (i == 0 || two)) {
@@ -364,40 +371,53 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         return __all_sync(0xffffffffu, wait(bar, parity, abort_flag)) != 0;
       };
       // the stage is free when both lanes' MMAs so far are done
-      auto release = [&](int t) {
-        mma_commit(empty_bar(t % C::kStages));
-        if (alone) mma_commit(empty_bar(t % C::kStages));
+      auto release = [&](int s) {
+        mma_commit(empty_bar(s));
+        if (alone) mma_commit(empty_bar(s));
       };
       auto qk = [&](int j) {  // scores of block j
-        const int t = copy_k(j);
-        if (!over(full_bar(t % C::kStages), phase(t))) return false;
+        const int s = stage(0, j);
+        if (!over(full_bar(s), phase(j))) return false;
         fence_after();
-        const uint64_t sk = sw128_desc(ring + (uint32_t)(t % C::kStages) * C::kTile);
+        const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             mma_f16(tm + 64 * (j & 1), qs + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
                     sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
           mma_commit(s_full(i, j & 1));
-          release(t);
+          release(s);
         }
         return true;
       };
       bool ok = over(q_full, 0);
       for (int j = 0; ok && j < min(nu, 2); ++j) ok = qk(j);
       for (int j = 0; ok && j < nu; ++j) {
-        const int t = copy_v(j);
-        ok = over(fixed_bar(j % C::kStages), (uint32_t)((j / C::kStages) & 1)) &&
-             over(p_full(i, j & 1), (uint32_t)((j >> 1) & 1));
-        if (!ok) break;
+        const int s = stage(1, j), kb = ks.block(j0 + j) * kKB;
+        if (!(ok = over(full_bar(s), phase(j)))) break;
+        if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
+          // rows that no row of the tile sees (both lanes' warps write the same zeros)
+          uint8_t* v = smem + C::kOffRing + s * C::kTile;
+          for (int r = lane; r < kKB; r += 32) {
+            const int key = kb + r;
+            if (!(key < ks.hi && (key >= ks.lo || key < ks.sink_end)))
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c)
+                *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        if (!(ok = over(p_full(i, j & 1), (uint32_t)((j >> 1) & 1)))) break;
         fence_after();
-        const uint64_t sv = sw128_desc_mn(ring + (uint32_t)(t % C::kStages) * C::kTile, C::kHalf);
+        const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kKB / 16; ++k)
             mma_ts(tm + 256, tm + 64 * (j & 1) + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
           mma_commit(pv_done(i));
-          release(t);
+          if (j == nu - 1) mma_commit(o_full(i));
+          release(s);
         }
         // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
         if (j + 2 < nu) ok = over(pv_done(i), (uint32_t)(j & 1)) && qk(j + 2);
@@ -412,27 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    // ------------------------------------------------ value rows nobody sees
-    // (it passes every value block on, so that it never falls a ring behind)
-    for (int j = 0; j < n; ++j) {
-      const int kb = ks.block(j0 + j) * kKB, t = copy_v(j), s = t % C::kStages;
-      if (!__all_sync(0xffffffffu, wait(full_bar(s), phase(t), abort_flag))) break;
-      if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
-        uint8_t* v = smem + C::kOffRing + s * C::kTile;
-        for (int r = lane; r < kKB; r += 32) {
-          const int key = kb + r;
-          if (!(key < ks.hi && (key >= ks.lo || key < ks.sink_end)))
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(fixed_bar(j % C::kStages));
-    }
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------ softmax and epilogue
     const int i = (warp - 4) >> 2, quad = warp & 3;  // TMEM lane quarter = warp & 3
     const int r = 32 * quad + lane;                  // row of the lane
@@ -560,9 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     // ---- epilogue
     const bool cut = pc.slot >= 0;
     if (i == 0 || two) {
-      // in order: the scores of the last block only say that the product three before the end is done
-      if (ok && n > 1) ok = wait(pv_done(i), (uint32_t)((n - 2) & 1), abort_flag);
-      if (ok && n > 0) ok = wait(pv_done(i), (uint32_t)((n - 1) & 1), abort_flag);
+      // (a barrier of its own: two products may be done since this warp last looked at pv_done)
+      if (ok && n > 0) ok = wait(o_full(i), 0, abort_flag);
       ok = __all_sync(0xffffffffu, ok) && (!cut || (pc.slot < a.slot_cap && pc.split < a.split_cap));
       fence_after();
       if (ok && cut) {
@@ -635,14 +634,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __syncthreads();
   fence_after();
   if (*abort_flag && threadIdx.x == 0) {
-    // copies still in flight land before the CTA exits: the queries and the last kStages
-    for (int t = max(0, issued_s - C::kStages) - 1; t < issued_s; ++t) {
-      const bool queries = t < max(0, issued_s - C::kStages);
+    // copies still in flight land before the CTA exits: the queries, and the
+    // last kDepth blocks of keys and values (an earlier one's stage was reused)
+    auto landed = [&](uint32_t bar, uint32_t parity) {
       const unsigned long long t0 = globaltimer();
-      while (!mbar_try(queries ? q_full : full_bar(t % C::kStages), queries ? 0u : phase(t)) &&
-             globaltimer() - t0 < kDrainWaitNs / 4) {
+      while (!mbar_try(bar, parity) && globaltimer() - t0 < kDrainWaitNs / 4) {
       }
-    }
+    };
+    if (n > 0) landed(q_full, 0);
+    for (int v = 0; v < 2; ++v)
+      for (int j = max(0, issued_s[v] - kDepth); j < issued_s[v]; ++j) landed(full_bar(stage(v, j)), phase(j));
   }
   __syncthreads();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
