@@ -181,13 +181,15 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[64]) {
+// 64 columns, waited for in the same statement.
+__device__ __forceinline__ void tmem_ld64_wait(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
       "%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,"
       "%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
-      "}, [%64];"
+      "}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
@@ -219,8 +221,12 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32])
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_wait(bar, parity, abort_flag, &g_paged_tc_status, &g_paged_tc_wait_ns);
+}
+// (the bounded loop stays out of the roles' code, which is long enough to be felt in the instruction cache)
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try(bar, parity) || wait_long(bar, parity, abort_flag);
 }
 
 template <typename T, int D>
@@ -457,8 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         float v[kKB];
         {
           uint32_t w[kKB];
-          tmem_ld(ts, w);
-          tmem_ld_wait(w);
+          tmem_ld64_wait(ts, w);
 #pragma unroll
           for (int x = 0; x < kKB; ++x) v[x] = __uint_as_float(w[x]);
         }
