@@ -18,12 +18,14 @@
 // the logits that looks for the n-th occurrence of its value.
 //
 // What bounds it: the row is read twice (the second time from L2) and counted
-// with one shared-memory atomic a token; the rest is latency. One cluster of
-// N CTAs serves a row: each counts its N-th of the row into its own 65536
-// 16-bit counters (128 KB of shared memory; a slice is kept to 65535 tokens so
-// that none overflows), then sums the N counts of its N-th of the values and
-// their masses, 32 values to a group; rank 0 gathers the 2048 groups, scans
-// them and cuts.
+// with one shared-memory atomic a token (about 7 cycles a warp of them); the
+// rest is latency. One cluster of N CTAs serves a row: each counts its N-th of
+// the row into its own 65536 16-bit counters (128 KB of shared memory; a slice
+// is kept to 65535 tokens so that none overflows), then sums the N counts of its
+// N-th of the values and their masses, 32 values to a group. Rank 0 gathers and
+// scans the 2048 groups, its first warp makes the cuts by searching the scanned
+// groups and then one group's 32 values, and the CTA whose slice holds the
+// token looks for it.
 #include <cooperative_groups.h>
 #include "ie_common.cuh"
 
@@ -90,9 +92,33 @@ struct Row {
   }
 };
 
-struct Found {
-  int key, rank;    // value and rank among its tokens
-  double w, before;  // its weight, the mass before the value
+// 2^x for x <= 0 in 64 bits: the nearest integer and the polynomial of degree 10
+// of least relative error (2.1e-16) on [-1/2, 1/2]. About a third of the library
+// exponential's instructions, and the 64-bit pipe is what masses wait for.
+__device__ __forceinline__ double exp2_neg(double x) {
+  if (!(x > -1000.0)) return 0.0;
+  const double big = 6755399441055744.0;  // 1.5 * 2^52
+  const double r = x + big;
+  const double f = x - (r - big);
+  double p = 7.037279530582804e-09;
+  p = fma(p, f, 1.0208537904552164e-07);
+  p = fma(p, f, 1.3215662831846104e-06);
+  p = fma(p, f, 1.5252658116561384e-05);
+  p = fma(p, f, 1.5403529961135955e-04);
+  p = fma(p, f, 1.3333558228561476e-03);
+  p = fma(p, f, 9.61812910803459e-03);
+  p = fma(p, f, 5.550410866445883e-02);
+  p = fma(p, f, 2.4022650695908768e-01);
+  p = fma(p, f, 6.931471805599497e-01);
+  p = fma(p, f, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));
+}
+
+// What rank 0 tells the others: the value and which of a slice's tokens of it.
+struct Pick {
+  int key, slice, rank;
+  int greedy;
+  double share;
 };
 
 template <typename T, int N>
@@ -101,15 +127,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   unsigned* hist = reinterpret_cast<unsigned*>(smem);  // two counters a word
   double* mass = reinterpret_cast<double*>(smem + kOffMass);
   int* count = reinterpret_cast<int*>(smem + kOffCount);
-  __shared__ int best_key;            // this CTA's smallest key (largest logit)
-  __shared__ long long above_min;     // its tokens with w >= min_p
+  __shared__ int best_key;   // this CTA's smallest key (largest logit)
+  __shared__ int above_min;  // its tokens with w >= min_p
   __shared__ double wsum[kWarps];
   __shared__ int csum[kWarps];
-  __shared__ int hit_group;
-  __shared__ long long hit_count;
-  __shared__ double hit_mass;
-  __shared__ Found found;
-  __shared__ long long kept;
+  __shared__ int hits[8][kWarps];
+  __shared__ Pick pick;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = N == 1 ? 0 : (int)cluster.block_rank();
@@ -139,14 +162,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   const int c0 = (int)((int64_t)in.chunks * rank / N), c1 = (int)((int64_t)in.chunks * (rank + 1) / N);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
   const bool greedy = !(temp > 0.f);
-  const double T64 = greedy ? 1.0 : (double)temp;
+  const double per = 1.4426950408889634 / (greedy ? 1.0 : (double)temp);  // log2 e / T
   const double low = a.min_p ? (double)a.min_p[row] : 0.0;
-  const double p = a.top_p ? (double)a.top_p[row] : 1.0;
-  const int k = a.top_k ? a.top_k[row] : 0;
   __syncthreads();
 
   // ---- count this slice's tokens by value
   int best = kKeys;
+#pragma unroll 2
   for (int c = c0 + t; c < c1; c += kThreads) {
     const uint4 x = in.load(c);
     const unsigned w[4] = {x.x, x.y, x.z, x.w};
@@ -162,59 +184,72 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   best = __reduce_min_sync(0xffffffffu, best);
   if (lane == 0) atomicMin(&best_key, best);
   sync_row();
+#pragma unroll
   for (int r = 0; r < N; ++r) best = min(best, *peer(&best_key, r));
   const double top = best < kKeys ? value_of<T>(best) : 0.0;
-  // weight of a value that occurs; +infinity as the largest logit takes it all
+  // weight of a value that occurs; an infinite largest logit takes it all
   auto weight = [&](int key) -> double {
     if (key == best) return 1.0;
     const double d = value_of<T>(key) - top;
-    return d < -1e300 ? 0.0 : exp(d / T64);
-  };
-  auto tokens = [&](int key) -> int {
-    int n = 0;
-#pragma unroll
-    for (int r = 0; r < N; ++r)
-      n += (peer(hist, r)[key >> 1] >> (16 * (key & 1))) & 0xFFFF;
-    return n;
+    return d < -1e300 ? 0.0 : exp2_neg(d * per);
   };
 
-  // ---- masses of this CTA's N-th of the values, 32 values (a warp) at a time
+  // ---- counts and masses of this CTA's N-th of the values: 8 a thread and
+  // step, 4 threads a group
   constexpr int kMine = kKeys / N;
-  long long above = 0;
-  for (int i = 0; i < kMine / kThreads; ++i) {
-    const int key = rank * kMine + i * kThreads + t;
-    const int n = tokens(key);
-    const unsigned any = __ballot_sync(0xffffffffu, n != 0);
-    double m = 0.0;
+  int above = 0;
+#pragma unroll 1
+  for (int i = 0; i < kMine / (8 * kThreads); ++i) {
+    const int key = rank * kMine + 8 * (i * kThreads + t);
+    uint4 x[N];
+#pragma unroll
+    for (int r = 0; r < N; ++r) x[r] = *reinterpret_cast<const uint4*>(peer(hist, r) + (key >> 1));
+    int n[8] = {};
     int cnt = 0;
-    if (any) {
-      cnt = __reduce_add_sync(0xffffffffu, n);
-      if (n) {
-        const double w = weight(key);
-        m = n * w;
-        if (w >= low) above += n;
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const unsigned w[4] = {x[r].x, x[r].y, x[r].z, x[r].w};
+#pragma unroll
+      for (int y = 0; y < 8; ++y) n[y] += (w[y >> 1] >> (16 * (y & 1))) & 0xFFFF;
+    }
+#pragma unroll
+    for (int y = 0; y < 8; ++y) cnt += n[y];
+    double m = 0.0;
+    if (__any_sync(0xffffffffu, cnt != 0)) {
+      if (cnt) {
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const double w = weight(key + y);
+          m += n[y] ? n[y] * w : 0.0;
+          above += n[y] && w >= low ? n[y] : 0;
+        }
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      for (int o = 1; o < 4; o <<= 1) {
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+        cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+      }
     }
-    if (lane == 0) {
+    if ((lane & 3) == 0) {
       mass[key >> 5] = m;
       count[key >> 5] = cnt;
     }
   }
-  if (above) atomicAdd(reinterpret_cast<unsigned long long*>(&above_min), (unsigned long long)above);
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0 && above) atomicAdd(&above_min, above);
   sync_row();
 
   if (rank == 0) {
-    // ---- scan the groups: thread t holds groups 2t and 2t + 1
+    // ---- scan the groups, thread t groups 2t and 2t + 1: mass[g] and count[g]
+    // become what lies before group g
     double m0, m1;
     int n0, n1;
     {
       const int r = (2 * t) / (kGroups / N);
-      const double* pm = peer(mass, r) + 2 * t;
-      const int* pc = peer(count, r) + 2 * t;
-      m0 = pm[0]; m1 = pm[1];
-      n0 = pc[0]; n1 = pc[1];
+      const double2 pm = *reinterpret_cast<const double2*>(peer(mass, r) + 2 * t);
+      const int2 pn = *reinterpret_cast<const int2*>(peer(count, r) + 2 * t);
+      m0 = pm.x; m1 = pm.y;
+      n0 = pn.x; n1 = pn.y;
     }
     double sm = m0 + m1;
     int sn = n0 + n1;
@@ -226,176 +261,220 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     }
     if (lane == 31) { wsum[warp] = sm; csum[warp] = sn; }
     __syncthreads();
-    double bm = 0.0, all_m = 0.0;
-    long long bn = 0, all_n = 0;
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) { bm += wsum[i]; bn += csum[i]; }
-      all_m += wsum[i];
-      all_n += csum[i];
+    // every warp scans the 32 warps' sums
+    double bm = wsum[lane];
+    int bn = csum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double um = __shfl_up_sync(0xffffffffu, bm, o);
+      const int un = __shfl_up_sync(0xffffffffu, bn, o);
+      if (lane >= o) { bm += um; bn += un; }
     }
-    // mass and tokens before each of the two groups, and after the second
-    const double e0 = bm + (sm - (m0 + m1)), e1 = bm + (sm - m1), e2 = bm + sm;
-    const long long f0 = bn + sn - n0 - n1, f1 = f0 + n0, f2 = f1 + n1;
+    const double all_m = __shfl_sync(0xffffffffu, bm, 31);
+    const int all_n = __shfl_sync(0xffffffffu, bn, 31);
+    bm = __shfl_sync(0xffffffffu, bm, max(warp - 1, 0));
+    bn = __shfl_sync(0xffffffffu, bn, max(warp - 1, 0));
+    if (warp == 0) { bm = 0.0; bn = 0; }
+    *reinterpret_cast<double2*>(mass + 2 * t) = make_double2(bm + (sm - (m0 + m1)), bm + (sm - m1));
+    *reinterpret_cast<int2*>(count + 2 * t) = make_int2(bn + sn - n0 - n1, bn + sn - n1);
+    __syncthreads();
 
-    // Each search below leaves one thread's group in shared memory and lets
-    // warp 0 find the value in it. `in0`, `in1`: the border lies in the group.
-    auto search = [&](bool in0, bool in1, auto inside) {
-      if (t == 0) hit_group = -1;
-      __syncthreads();
-      // the first group that holds the border (rounding may let two claim it)
-      if (in0) atomicMax(&hit_group, kGroups - 2 * t);
-      else if (in1) atomicMax(&hit_group, kGroups - 2 * t - 1);
-      __syncthreads();
-      const int g = kGroups - hit_group;
-      if (hit_group > 0 && (g >> 1) == t) {
-        hit_mass = (g & 1) ? e1 : e0;
-        hit_count = (g & 1) ? f1 : f0;
-      }
-      __syncthreads();
-      if (warp == 0 && hit_group > 0) {
-        const int key = 32 * g + lane;
-        const int n = tokens(key);
-        const double w = n ? weight(key) : 0.0, mass_before = hit_mass;
-        const long long count_before = hit_count;
-        double m = n * w;
-        int c = n;
+    if (warp == 0) {
+      // The values of one group, one a lane: tokens, weight, what lies before.
+      struct Lane {
+        int key, n, before_n;
+        double w, before_m;
+      };
+      auto tokens = [&](int key) {
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < N; ++r) n += (peer(hist, r)[key >> 1] >> (16 * (key & 1))) & 0xFFFF;
+        return n;
+      };
+      auto values = [&](int g) {
+        Lane v;
+        v.key = 32 * g + lane;
+        v.n = tokens(v.key);
+        v.w = v.n ? weight(v.key) : 0.0;
+        double m = v.n * v.w;
+        int c = v.n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const double um = __shfl_up_sync(0xffffffffu, m, o);
           const int uc = __shfl_up_sync(0xffffffffu, c, o);
           if (lane >= o) { m += um; c += uc; }
         }
-        inside(key, n, w, mass_before + (m - n * w), count_before + c - n);
-      }
-      __syncthreads();
-      return hit_group > 0;
-    };
-    // mass of the first n tokens, 1 <= n < all_n (all threads)
-    auto mass_of_first = [&](long long n) -> double {
-      search(f0 < n && n <= f1, f1 < n && n <= f2, [&](int, int c, double w, double before, long long cb) {
-        if (c && cb < n && n <= cb + c) hit_mass = before + (double)(n - cb) * w;
-      });
-      return hit_mass;
-    };
-
-    if (all_n == 0) {
-      if (t == 0) {
-        a.idx[row] = -1;
-        if (a.logprob) a.logprob[row] = __int_as_float(0xff800000);
-      }
-    } else {
-      long long L = all_n;
-      double Z = all_m;
-      if (greedy) {
-        L = 1;
-      } else {
-        if (k > 0 && k < L) {
-          L = k;
-          if (p < 1.0) Z = mass_of_first(L);
-        }
-        if (!(p >= 1.0)) {
-          // the first value that holds a token with mass >= target before it
-          // or right after its last one: its tokens before the target are kept
-          const double target = p * Z;
-          if (t == 0) kept = L;
-          const bool some = search(m0 > 0.0 && e1 >= target, m1 > 0.0 && e2 >= target,
-                                   [&](int, int c, double w, double before, long long cb) {
-            const bool over = c && before + c * w >= target;
-            const unsigned who = __ballot_sync(0xffffffffu, over);
-            if (!who && lane == 31) kept = cb + c;  // by a rounding: the border is the group's end
-            if (who && lane == __ffs(who) - 1) {
-              long long n = w > 0.0 ? (long long)ceil(fmin(fmax((target - before) / w, 0.0), (double)c)) : c;
-              while (n > 0 && before + (double)(n - 1) * w >= target) --n;
-              while (n < c && before + (double)n * w < target) ++n;
-              kept = cb + n;
-            }
-          });
-          if (some && kept < L) L = kept;
-          if (p != p) L = 1;
-        }
-        long long m = 0;
-        for (int r = 0; r < N; ++r) m += *peer(&above_min, r);
-        if (m < L) L = m;
-        if (L < 1) L = 1;
-      }
-      Z = L < all_n ? mass_of_first(L) : all_m;
-      const double target = (greedy ? 0.0 : (double)a.u[row]) * Z;
-      if (t == 0) found.key = -1;
-      search(n0 && e1 > target, n1 && e2 > target, [&](int key, int c, double w, double before, long long cb) {
-        const bool over = c && before + c * w > target;
-        const unsigned who = __ballot_sync(0xffffffffu, over), any = __ballot_sync(0xffffffffu, c != 0);
-        // by a rounding none may pass it: then the group's last token does
-        if (any && lane == (who ? __ffs(who) - 1 : 31 - __clz(any))) {
-          long long n = (long long)fmin(fmax((target - before) / w, 0.0), (double)(c - 1));
-          while (n > 0 && before + (double)n * w > target) --n;
-          while (n < c - 1 && before + (double)(n + 1) * w <= target) ++n;
-          if (cb + n < L) {
-            found.key = key;
-            found.rank = (int)n;
-            found.w = w;
-          }
-        }
-      });
-      // u * Z reached the end of the kept mass (u >= 1, or rounding): the last kept token
-      if (found.key < 0) {
-        __syncthreads();
-        search(f0 < L && L <= f1, f1 < L && L <= f2, [&](int key, int c, double w, double, long long cb) {
-          if (c && cb < L && L <= cb + c) {
-            found.key = key;
-            found.rank = (int)(L - cb - 1);
-            found.w = w;
-          }
-        });
-      }
-      // ---- the found.rank-th token of that value in index order
-      const int key = found.key;
-      int left = found.rank, slice = 0;
-      for (; slice < N - 1; ++slice) {
-        const int n = (peer(hist, slice)[key >> 1] >> (16 * (key & 1))) & 0xFFFF;
-        if (left < n) break;
-        left -= n;
-      }
-      const int s0 = (int)((int64_t)in.chunks * slice / N), s1 = (int)((int64_t)in.chunks * (slice + 1) / N);
-      const int each = (s1 - s0 + kThreads - 1) / kThreads;
-      const int b0 = s0 + t * each, b1 = min(b0 + each, s1);
-      int mine = 0;
-      auto matches = [&](const uint4& x) {
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-        unsigned hits = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key_of<T>((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) == key) hits |= 1u << i;
-        return hits;
+        v.before_m = mass[g] + (m - v.n * v.w);
+        v.before_n = count[g] + c - v.n;
+        return v;
       };
-      for (int c = b0; c < b1; ++c) mine += __popc(matches(in.load(c)));
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
-      }
-      if (lane == 31) csum[warp] = sum;
-      __syncthreads();
-      for (int i = 0; i < warp; ++i) sum += csum[i];
-      int skip = left - (sum - mine);  // this thread's matches to pass over
-      if (skip >= 0 && skip < mine) {
-        for (int c = b0; c < b1; ++c) {
-          unsigned h = matches(in.load(c));
-          const int n = __popc(h);
-          if (skip >= n) {
-            skip -= n;
-            continue;
+      // first group whose end passes the border; ends(g) is what lies before g
+      auto group_of = [&](auto passes) {
+        const int s = __ffs(__ballot_sync(0xffffffffu, passes(64 * (lane + 1)))) - 1;
+        if (s < 0) return kGroups - 1;
+        const unsigned odd = __ballot_sync(0xffffffffu, passes(64 * s + 2 * lane + 1));
+        const unsigned even = __ballot_sync(0xffffffffu, passes(64 * s + 2 * lane + 2));
+        const int f = __ffs(even) - 1;
+        return 64 * s + 2 * f + ((odd >> f) & 1 ? 0 : 1);
+      };
+      auto count_at = [&](int g) { return g < kGroups ? count[g] : all_n; };
+      auto mass_at = [&](int g) { return g < kGroups ? mass[g] : all_m; };
+      // mass of the first n tokens, 1 <= n <= all_n
+      auto mass_of_first = [&](int n) {
+        if (n >= all_n) return all_m;
+        const Lane v = values(group_of([&](int g) { return count_at(g) >= n; }));
+        const int who = __ffs(__ballot_sync(0xffffffffu, v.before_n + v.n >= n)) - 1;
+        return __shfl_sync(0xffffffffu, v.before_m + (double)(n - v.before_n) * v.w, max(who, 0));
+      };
+      Pick out = {-1, 0, 0, greedy, 0.0};
+      if (all_n > 0) {
+        int L = all_n;
+        double Z = all_m;
+        if (greedy) {
+          L = 1;
+          Z = 1.0;
+        } else {
+          const double p = a.top_p ? (double)a.top_p[row] : 1.0;
+          const int k = a.top_k ? a.top_k[row] : 0;
+          if (k > 0 && k < L) {
+            L = k;
+            Z = mass_of_first(L);
           }
-          for (; skip > 0; --skip) h &= h - 1;
-          a.idx[row] = 8 * c - in.lead + __ffs(h) - 1;
-          if (a.logprob) a.logprob[row] = greedy ? 0.f : (float)log(found.w / Z);
-          break;
+          if (!(p >= 1.0)) {
+            // a token is kept while the mass before it is below the border
+            const double border = p * Z;
+            const Lane v = values(group_of([&](int g) { return mass_at(g) >= border; }));
+            const unsigned over = __ballot_sync(0xffffffffu, v.n && v.before_m + v.n * v.w >= border);
+            const int who = over ? __ffs(over) - 1 : 31;  // none by a rounding: the border is the group's end
+            int n = v.n;
+            if (over && v.w > 0.0) {
+              n = (int)ceil(fmin(fmax((border - v.before_m) / v.w, 0.0), (double)v.n));
+              while (n > 0 && v.before_m + (double)(n - 1) * v.w >= border) --n;
+              while (n < v.n && v.before_m + (double)n * v.w < border) ++n;
+            }
+            const int kept = max(__shfl_sync(0xffffffffu, v.before_n + n, who), 1);
+            const double mk = __shfl_sync(0xffffffffu, v.before_m + (double)n * v.w, who);
+            if (p != p) {
+              L = 1;
+              Z = 1.0;
+            } else if (kept < L) {
+              L = kept;
+              Z = kept == 1 ? 1.0 : mk;
+            }
+          }
+          int m = 0;
+          if (a.min_p) {
+#pragma unroll
+            for (int r = 0; r < N; ++r) m += *peer(&above_min, r);
+            if (m < 1) m = 1;
+            if (m < L) {
+              L = m;
+              Z = mass_of_first(L);
+            }
+          }
+        }
+        const double border = greedy ? 0.0 : (double)a.u[row] * Z;
+        Lane v = values(group_of([&](int g) { return mass_at(g) > border; }));
+        const unsigned any = __ballot_sync(0xffffffffu, v.n != 0);
+        const unsigned over = __ballot_sync(0xffffffffu, v.n && v.before_m + v.n * v.w > border);
+        // none by a rounding: the group's last token
+        int who = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
+        int n = (int)fmin(fmax((border - v.before_m) / v.w, 0.0), (double)max(v.n - 1, 0));
+        if (v.w > 0.0) {
+          while (n > 0 && v.before_m + (double)n * v.w > border) --n;
+          while (n < v.n - 1 && v.before_m + (double)(n + 1) * v.w <= border) ++n;
+        }
+        if (__shfl_sync(0xffffffffu, v.n == 0 || !(border < Z) || v.before_n + n >= L, who)) {
+          // u * Z reached the end of the kept mass: the last kept token
+          v = values(group_of([&](int g) { return count_at(g) >= L; }));
+          who = __ffs(__ballot_sync(0xffffffffu, v.before_n + v.n >= L)) - 1;
+          n = L - 1 - v.before_n;
+        }
+        out.key = __shfl_sync(0xffffffffu, v.key, who);
+        out.rank = __shfl_sync(0xffffffffu, n, who);
+        out.share = __shfl_sync(0xffffffffu, v.w, who) / Z;
+        // the slice that holds that one of the value's tokens
+#pragma unroll
+        for (int r = 0; r < N - 1; ++r) {
+          const int c = (peer(hist, r)[out.key >> 1] >> (16 * (out.key & 1))) & 0xFFFF;
+          if (out.slice == r && out.rank >= c) {
+            out.rank -= c;
+            ++out.slice;
+          }
         }
       }
+      if (lane < N) *peer(&pick, lane) = out;
     }
   }
-  // the peers' shared memory stays until rank 0 has read it
-  if constexpr (N > 1) cluster.sync();
+  sync_row();
+
+  // ---- that token of the slice, in index order: chunks go by (step, thread)
+  const Pick out = pick;
+  if (out.key < 0) {
+    if (rank == 0 && t == 0) {
+      a.idx[row] = -1;
+      if (a.logprob) a.logprob[row] = __int_as_float(0xff800000);
+    }
+    return;
+  }
+  if (rank != out.slice) return;
+  auto matches = [&](int i) -> unsigned {
+    const int c = c0 + i * kThreads + t;
+    if (c >= c1) return 0u;
+    const uint4 x = in.load(c);
+    const unsigned w[4] = {x.x, x.y, x.z, x.w};
+    unsigned h = 0;
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+      if (key_of<T>((w[y >> 1] >> (16 * (y & 1))) & 0xFFFFu) == out.key) h |= 1u << y;
+    return h;
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // a slice has at most 8 kThreads chunks
+    const int n = __reduce_add_sync(0xffffffffu, __popc(matches(i)));
+    if (lane == 0) hits[i][warp] = n;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    // lane l scans the 8 entries 8 l .. of the 256 (step, warp) counts
+    int mine[8], sum = 0;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      mine[y] = hits[lane >> 2][8 * (lane & 3) + y];
+      sum += mine[y];
+    }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
+    }
+    before -= sum;
+    if (out.rank >= before && out.rank < before + sum) {
+      int y = 0, left = out.rank - before;
+      while (left >= mine[y]) left -= mine[y++];
+      csum[0] = lane >> 2;              // the step
+      csum[1] = 8 * (lane & 3) + y;     // the warp
+      csum[2] = left;
+    }
+  }
+  __syncthreads();
+  if (warp == csum[1]) {
+    unsigned h = matches(csum[0]);
+    const int n = __popc(h);
+    int before = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
+    }
+    int skip = csum[2] - (before - n);
+    if (skip >= 0 && skip < n) {
+      for (; skip > 0; --skip) h &= h - 1;
+      a.idx[row] = 8 * (c0 + csum[0] * kThreads + t) - in.lead + __ffs(h) - 1;
+      if (a.logprob) a.logprob[row] = out.greedy ? 0.f : (float)log(out.share);
+    }
+  }
 }
 
 template <typename T, int N>
