@@ -413,7 +413,7 @@ int ie_argmax(ie_dtype dt, int M, int V, const void* logits, int64_t ld,
  * on an order of summation. -infinity and NaN logits are never sampled;
  * a row without others gives idx -1 and logprob -infinity. The tie order
  * differs from ie_argmax's, which follows the reference's tree.
- * V at most 524160 (IE_ERR_UNSUPPORTED above). */
+ * V at most 524159 (IE_ERR_UNSUPPORTED above). */
 int ie_sample(ie_dtype dt, int M, int V, const void* logits, int64_t ld,
               const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* u,
               int* idx_out, float* logprob_out, void* stream);

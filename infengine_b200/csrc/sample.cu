@@ -66,31 +66,37 @@ __device__ __forceinline__ int key_of(unsigned b) {
   const unsigned up = (b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u);
   return (int)(0xFFFFu - up);
 }
+__device__ __forceinline__ unsigned bits_of(int key) {
+  const unsigned up = 0xFFFFu - (unsigned)key;
+  return (up & 0x8000u) ? (up & 0x7FFFu) : (~up & 0xFFFFu);
+}
 template <typename T>
 __device__ __forceinline__ double value_of(int key) {
-  const unsigned up = 0xFFFFu - (unsigned)key;
-  const unsigned short b = (unsigned short)((up & 0x8000u) ? (up & 0x7FFFu) : (~up & 0xFFFFu));
+  const unsigned short b = (unsigned short)bits_of(key);
   T v;
   memcpy(&v, &b, 2);
   return (double)DT<T>::to_f(v);
 }
 
-// The row cut into 16-byte aligned chunks of 8: chunk c holds tokens
-// 8c - lead .. 8c - lead + 7, of which the first and last chunk may lack some.
-struct Row {
-  const unsigned short* first;  // address of chunk 0 (not read below the row)
-  int lead, V, chunks;
-  __device__ __forceinline__ uint4 load(int c) const {
-    const int i0 = 8 * c - lead;
-    if (i0 >= 0 && i0 + 8 <= V) return __ldg(reinterpret_cast<const uint4*>(first) + c);
-    unsigned short e[8];
+// Distance from a value of this 16-bit pattern to its neighbours (the 8 aligned
+// values around it are equally spaced).
+template <typename T>
+__device__ __forceinline__ double spacing_of(int key) {
+  const unsigned up = 0xFFFFu - (unsigned)key, b = (up & 0x8000u) ? up & 0x7FFFu : ~up & 0x7FFFu;
+  constexpr int kMant = DT<T>::id == IE_DTYPE_BF16 ? 7 : 10, kBias = DT<T>::id == IE_DTYPE_BF16 ? 127 : 15;
+  const int e = max((int)(b >> kMant), 1) - kBias - kMant;
+  return __hiloint2double((1023 + e) << 20, 0);
+}
+
+// K of the 16-byte chunks c, c + step .. (0xFFFF, a NaN in both types, from
+// `end` on), all loads in flight at once.
+template <int K>
+__device__ __forceinline__ void load_chunks(const uint4* p, int c, int step, int end, uint4 (&x)[K]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i0 + i >= 0 && i0 + i < V ? __ldg(first + 8 * c + i) : (unsigned short)0xFFFFu;
-    uint4 r;  // 0xFFFF is a NaN in both types: skipped
-    memcpy(&r, e, 16);
-    return r;
-  }
-};
+  for (int i = 0; i < K; ++i)
+    x[i] = c + i * step < end ? __ldg(p + c + i * step)
+                              : make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
+}
 
 // 2^x for x <= 0 in 64 bits: the nearest integer and the polynomial of degree 10
 // of least relative error (2.1e-16) on [-1/2, 1/2]. About a third of the library
@@ -137,29 +143,33 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = N == 1 ? 0 : (int)cluster.block_rank();
   const int row = blockIdx.x / N, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  auto sync_row = [&] {
-    if constexpr (N == 1) __syncthreads();
-    else cluster.sync();
-  };
+  // (also for a cluster of one: with __syncthreads in its place the one-warp
+  // part ran four times slower)
+  auto sync_row = [&] { cluster.sync(); };
   auto peer = [&](auto* p, int r) {
     if constexpr (N == 1) return p;
     else return cluster.map_shared_rank(p, r);
   };
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const unsigned short* base = static_cast<const unsigned short*>(a.logits) + (int64_t)row * a.ld;
+  // The row as up to 7 tokens before the first 16-byte boundary (slice 0's),
+  // chunks of 8, of which this slice has c0 .. c1 - 1, and up to 7 tokens
+  // behind them (the last slice's).
+  const int head = min((int)((0u - (unsigned)reinterpret_cast<uintptr_t>(base)) & 15u) >> 1, a.V);
+  const int chunks = (a.V - head) >> 3, tail0 = head + 8 * chunks;
+  const uint4* body = reinterpret_cast<const uint4*>(base + head);
+  const int c0 = (int)((int64_t)chunks * rank / N), c1 = (int)((int64_t)chunks * (rank + 1) / N);
+  // the first chunks are on their way while the counters are cleared
+  constexpr int kAhead = 2;
+  uint4 x[kAhead];
+  load_chunks(body, c0 + t, kThreads, c1, x);
   for (int i = t; i < kHistBytes / 16; i += kThreads) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   if (t == 0) {
     best_key = kKeys;
     above_min = 0;
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const unsigned short* base = static_cast<const unsigned short*>(a.logits) + (int64_t)row * a.ld;
-  Row in;
-  in.lead = (int)((reinterpret_cast<uintptr_t>(base) & 15u) >> 1);
-  in.first = base - in.lead;
-  in.V = a.V;
-  in.chunks = (in.lead + a.V + 7) >> 3;
-  const int c0 = (int)((int64_t)in.chunks * rank / N), c1 = (int)((int64_t)in.chunks * (rank + 1) / N);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
   const bool greedy = !(temp > 0.f);
   const double per = 1.4426950408889634 / (greedy ? 1.0 : (double)temp);  // log2 e / T
@@ -168,18 +178,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
 
   // ---- count this slice's tokens by value
   int best = kKeys;
-#pragma unroll 2
-  for (int c = c0 + t; c < c1; c += kThreads) {
-    const uint4 x = in.load(c);
-    const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = key_of<T>((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-      if (key >= 0) {
-        best = min(best, key);
-        atomicAdd(hist + (key >> 1), 1u << (16 * (key & 1)));
-      }
+  auto take = [&](unsigned bits) {
+    const int key = key_of<T>(bits);
+    if (key >= 0) {
+      best = min(best, key);
+      atomicAdd(hist + (key >> 1), 1u << (16 * (key & 1)));
     }
+  };
+  if (rank == 0 && t < head) take(__ldg(base + t));
+  if (rank == N - 1 && t < a.V - tail0) take(__ldg(base + tail0 + t));
+  for (int c = c0 + t; c < c1;) {
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const unsigned w[4] = {x[y].x, x[y].y, x[y].z, x[y].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) take((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+    }
+    c += kAhead * kThreads;
+    load_chunks(body, c, kThreads, c1, x);
   }
   best = __reduce_min_sync(0xffffffffu, best);
   if (lane == 0) atomicMin(&best_key, best);
@@ -217,11 +233,17 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     double m = 0.0;
     if (__any_sync(0xffffffffu, cnt != 0)) {
       if (cnt) {
+        // equally spaced values: each weight is the last one times r
+        const double r = exp2_neg(-spacing_of<T>(key) * per);
+        double w = best >= key && best < key + 8 ? 0.0 : weight(key);
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-          const double w = weight(key + y);
-          m += n[y] ? n[y] * w : 0.0;
-          above += n[y] && w >= low ? n[y] : 0;
+          if (key + y == best) w = 1.0;
+          // n as a double: its bits below 2^52, without the slow conversion
+          const double dn = __hiloint2double(0x43300000, n[y]) - 4503599627370496.0;
+          m += n[y] ? dn * w : 0.0;
+          if (low > 0.0) above += n[y] && w >= low ? n[y] : 0;
+          w *= r;
         }
       }
 #pragma unroll
@@ -363,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
             }
           }
           int m = 0;
-          if (a.min_p) {
+          if (low > 0.0 || low != low) {
 #pragma unroll
             for (int r = 0; r < N; ++r) m += *peer(&above_min, r);
             if (m < 1) m = 1;
@@ -418,20 +440,35 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     return;
   }
   if (rank != out.slice) return;
-  auto matches = [&](int i) -> unsigned {
-    const int c = c0 + i * kThreads + t;
-    if (c >= c1) return 0u;
-    const uint4 x = in.load(c);
-    const unsigned w[4] = {x.x, x.y, x.z, x.w};
-    unsigned h = 0;
+  // tokens of the value in a chunk: equal bits, or either zero
+  const unsigned bits = bits_of(out.key), both = bits | bits << 16;
+  const unsigned care = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;
+  auto matches = [&](const uint4& x) -> unsigned {
+    const unsigned w[4] = {(x.x ^ both) & care, (x.y ^ both) & care, (x.z ^ both) & care, (x.w ^ both) & care};
+    unsigned any = 0;  // never 0 when a half word is
 #pragma unroll
-    for (int y = 0; y < 8; ++y)
-      if (key_of<T>((w[y >> 1] >> (16 * (y & 1))) & 0xFFFFu) == out.key) h |= 1u << y;
+    for (int y = 0; y < 4; ++y) any |= (w[y] - 0x00010001u) & ~w[y];
+    unsigned h = 0;
+    if (any & 0x80008000u)
+#pragma unroll
+      for (int y = 0; y < 8; ++y)
+        if (((w[y >> 1] >> (16 * (y & 1))) & 0xFFFFu) == 0u) h |= 1u << y;
     return h;
   };
+  auto write = [&](int id) {
+    a.idx[row] = id;
+    if (a.logprob) a.logprob[row] = out.greedy ? 0.f : (float)log(out.share);
+  };
+  unsigned found[8];  // a slice has at most 8 kThreads chunks
+  {
+    uint4 y[8];
+    load_chunks(body, c0 + t, kThreads, c1, y);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {  // a slice has at most 8 kThreads chunks
-    const int n = __reduce_add_sync(0xffffffffu, __popc(matches(i)));
+    for (int i = 0; i < 8; ++i) found[i] = c0 + i * kThreads < c1 ? matches(y[i]) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = __reduce_add_sync(0xffffffffu, __popc(found[i]));
     if (lane == 0) hits[i][warp] = n;
   }
   __syncthreads();
@@ -449,18 +486,45 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
       const int u = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += u;
     }
+    const int all = __shfl_sync(0xffffffffu, before, 31);
     before -= sum;
-    if (out.rank >= before && out.rank < before + sum) {
-      int y = 0, left = out.rank - before;
-      while (left >= mine[y]) left -= mine[y++];
-      csum[0] = lane >> 2;              // the step
-      csum[1] = 8 * (lane & 3) + y;     // the warp
+    // the tokens outside the chunks, one a lane: those before and those behind
+    const int i0 = min(lane, a.V - 1), i1 = min(tail0 + lane, a.V - 1);
+    const unsigned first =
+        __ballot_sync(0xffffffffu, rank == 0 && lane < head && key_of<T>(__ldg(base + i0)) == out.key);
+    const unsigned last =
+        __ballot_sync(0xffffffffu, rank == N - 1 && tail0 + lane < a.V && key_of<T>(__ldg(base + i1)) == out.key);
+    int left = out.rank;
+    auto nth = [](unsigned m, int n) {
+      for (; n > 0; --n) m &= m - 1;
+      return __ffs(m) - 1;
+    };
+    if (lane == 0) csum[1] = -1;
+    __syncwarp();
+    if (left < __popc(first)) {
+      if (lane == 0) write(nth(first, left));
+    } else if ((left -= __popc(first)) >= all) {
+      if (lane == 0) write(tail0 + nth(last, left - all));
+    } else if (left >= before && left < before + sum) {
+      left -= before;
+      int y = 0;
+#pragma unroll
+      for (int z = 0; z < 7; ++z)
+        if (y == z && left >= mine[z]) {
+          left -= mine[z];
+          y = z + 1;
+        }
+      csum[0] = lane >> 2;           // the step
+      csum[1] = 8 * (lane & 3) + y;  // the warp
       csum[2] = left;
     }
   }
   __syncthreads();
   if (warp == csum[1]) {
-    unsigned h = matches(csum[0]);
+    unsigned h = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == csum[0]) h = found[i];
     const int n = __popc(h);
     int before = n;
 #pragma unroll
@@ -471,8 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     int skip = csum[2] - (before - n);
     if (skip >= 0 && skip < n) {
       for (; skip > 0; --skip) h &= h - 1;
-      a.idx[row] = 8 * (c0 + csum[0] * kThreads + t) - in.lead + __ffs(h) - 1;
-      if (a.logprob) a.logprob[row] = out.greedy ? 0.f : (float)log(out.share);
+      write(head + 8 * (c0 + csum[0] * kThreads + t) + __ffs(h) - 1);
     }
   }
 }
@@ -507,7 +570,7 @@ template <typename T>
 int dispatch(const SampleArgs& a, int M, cudaStream_t st) {
   // As many CTAs a row as keep the rows within one wave of the 148 SMs, at
   // least as many as the 16-bit counters need.
-  auto fits = [&](int n) { return ((int64_t)a.V + 14) / 8 / n + 1 <= kMaxSlice / 8; };
+  auto fits = [&](int n) { return (int64_t)a.V / 8 / n + 1 <= (kMaxSlice - 14) / 8; };
   if (!fits(8)) return IE_ERR_UNSUPPORTED;
   if (M * 8 <= 148 || !fits(4)) return launch<T, 8>(a, M, st);
   if (M * 4 <= 148 || !fits(2)) return launch<T, 4>(a, M, st);
