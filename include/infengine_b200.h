@@ -325,10 +325,10 @@ int ie_qk_norm_rope_paged(ie_dtype dt, int B, int T, int n_q_heads,
  * A cache row that no row of its sequence sees (behind kv_len, outside every
  * window) may hold anything. Rows that are seen must be finite where another
  * row of the same sequence does not see them: 0 * infinity is not 0.
- * workspace: ie_paged_attention_workspace_size() bytes, 16-byte aligned,
- * needing no initialisation and no state between calls; calls that share one
- * must not overlap on the GPU (one stream, or ordered streams, and not two
- * captured graphs that may run at once). The same call gives the same bits
+ * workspace: ie_paged_attention_workspace_size() bytes, 16-byte aligned, its
+ * first 64 KB zeroed once when allocated; every call leaves them zeroed again.
+ * Calls that share one must not overlap on the GPU (one stream, or ordered
+ * streams, and not two captured graphs that may run at once). The same call gives the same bits
  * every time; a row's last bits may depend on the other sequences of the
  * batch, which decide how the work is divided. */
 size_t ie_paged_attention_workspace_size(void);

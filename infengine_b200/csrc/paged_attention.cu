@@ -1,5 +1,5 @@
-// Attention of new tokens over a paged cache: entry point, the kernel for few
-// rows, and the kernel that joins split tiles.
+// Attention of new tokens over a paged cache: entry point and the kernel for
+// few rows.
 //
 //   x_j = scale * q . k_j        keys j <= position with (position - j < window or j < sinks)
 //   o   = sum_j e^(x_j - m) v_j / sum_j e^(x_j - m)       zeros where no key is seen
@@ -20,6 +20,9 @@
 // as m16n8k16 with the rows as M, and no barrier is shared between warps until
 // the four warps' outputs meet at the end. 96 KB of ring a CTA, two CTAs an SM:
 // 192 KB of copies in flight an SM, above the ~50 KB that HBM latency needs.
+// The CTA that finishes a cut tile's last piece joins the pieces in their order:
+// with M = max_s m_s the output is sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s
+// (a joining kernel in its place cost a decode step of one row 3 us more).
 //
 // A block's box is copied only if some row of the tile sees one of its keys, so
 // table entries outside the visible range are never followed; visible range's
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   __shared__ __align__(8) uint64_t bars[kWarps * kSlots];
   __shared__ Scan scan;
   __shared__ float sm_m[kWarps][kMT], sm_l[kWarps][kMT];
-  __shared__ int abort_s;
+  __shared__ int abort_s, last_s;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 32) {
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (!find_piece<kKB, kThreads, false>(a, blockIdx.x, scan, &g_paged_attn_status)) return;
+  if (!find_piece<kKB, kThreads>(a, blockIdx.x, scan, &g_paged_attn_status)) return;
   const Piece pc = scan.p;
   const Seq sq = scan.seq;
   const int rows = sq.tokens * a.group;
@@ -137,9 +140,10 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
   const int tok0 = row0 / a.group, tok1 = (row0 + nrows - 1) / a.group;
   const Keys ks = tile_keys<kKB>(a, sq, tok0, tok1);
   const int nb = ks.blocks();
-  const int p0 = (int)((int64_t)nb * pc.piece / pc.pieces), p1 = (int)((int64_t)nb * (pc.piece + 1) / pc.pieces);
-  const int j0 = p0 + (int)((int64_t)(p1 - p0) * warp / kWarps);
-  const int n = p0 + (int)((int64_t)(p1 - p0) * (warp + 1) / kWarps) - j0;
+  int p0, np, j0, n;  // the piece's blocks, this warp's
+  piece_range(nb, pc.pieces, pc.piece, p0, np);
+  piece_range(np, kWarps, warp, j0, n);
+  j0 += p0;
 
   uint8_t* ring = smem + warp * kRingBytes;
   const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(bars + warp * kSlots);
@@ -357,138 +361,130 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     }
   }
   __syncthreads();
-  if (abort_s) return;
+  const bool cut = pc.slot >= 0 && pc.slot < a.slot_cap && pc.split < a.split_cap;
+  bool good = !abort_s && (cut || pc.slot < 0);
   float* acc = reinterpret_cast<float*>(ring);  // [16][D], this warp's
+  // 16-byte columns of the rows a quad writes together are spread over the banks
+  auto at = [&](int r, int d) { return r * D + (d ^ (8 * (r & 3))); };
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int r = g + 8 * x;
-    float top = sm_m[0][r];
+  for (int x = 0; x < 2; ++x)
+    if (8 * x < nrows) {
+      const int r = g + 8 * x;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-    const float f = top == -INFINITY ? 0.f : ex2(m[x] - top);
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-      *reinterpret_cast<float2*>(acc + r * D + ((8 * i + 2 * tq) ^ (8 * (r & 3)))) =
-          make_float2(o[i][2 * x] * f, o[i][2 * x + 1] * f);
-  }
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<float2*>(acc + at(r, 8 * i + 2 * tq)) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
+    }
   __syncthreads();
-  const bool cut = pc.slot >= 0;
-  if (cut && (pc.slot >= a.slot_cap || pc.split >= a.split_cap)) return;
   constexpr int kPer = kMT * D / kThreads;  // consecutive outputs of a thread
   const int r = tid / (D / kPer), d0 = (tid % (D / kPer)) * kPer;
-  if (r < nrows) {
-    float top = sm_m[0][r], sum = 0.f;
+  float v[kPer], top = sm_m[0][r], sum = 0.f;
+  // the warps' parts of this thread's outputs at their common maximum, in warp order
+  auto add_up = [&] {
+    top = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
+    sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+    for (int i = 0; i < kPer; ++i) v[i] = 0.f;
+#pragma unroll 1
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = top == -INFINITY ? 0.f : ex2(sm_m[w][r] - top);
+      sum += f * sm_l[w][r];
+      const float* p = reinterpret_cast<const float*>(smem + w * kRingBytes);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += top == -INFINITY ? 0.f : sm_l[w][r] * ex2(sm_m[w][r] - top);
-    float v[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; i += 4) {
-      float4 t4 = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * kRingBytes) +
-                                                          r * D + ((d0 + i) ^ (8 * (r & 3))));
-        t4.x += u.x; t4.y += u.y; t4.z += u.z; t4.w += u.w;
+      for (int i = 0; i < kPer; i += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p + at(r, d0 + i));
+        v[i] += f * u.x;
+        v[i + 1] += f * u.y;
+        v[i + 2] += f * u.z;
+        v[i + 3] += f * u.w;
       }
-      v[i] = t4.x; v[i + 1] = t4.y; v[i + 2] = t4.z; v[i + 3] = t4.w;
     }
-    if (cut) {
+  };
+  if (good && r < nrows) add_up();
+  if (cut) {
+    if (good && r < nrows) {
       float* po = a.part_o + ((int64_t)pc.slot * kMT + r) * D + d0;
 #pragma unroll
       for (int i = 0; i < kPer; i += 4)
-        *reinterpret_cast<float4*>(po + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-      if (d0 == 0) a.part_ml[(int64_t)pc.slot * kMT + r] = make_float2(top, sum);
-    } else {
-      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-      const int tok = (row0 + r) / a.group;
-      T* dst = static_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.ld_out +
-               (int64_t)(pc.head * a.group + (row0 + r) % a.group) * D + d0;
-#pragma unroll
-      for (int i = 0; i < kPer; i += 8) {
-        uint4 w;
-        w.x = pack2<T>(v[i] * inv, v[i + 1] * inv);
-        w.y = pack2<T>(v[i + 2] * inv, v[i + 3] * inv);
-        w.z = pack2<T>(v[i + 4] * inv, v[i + 5] * inv);
-        w.w = pack2<T>(v[i + 6] * inv, v[i + 7] * inv);
-        *reinterpret_cast<uint4*>(dst + i) = w;
-      }
+        __stcg(reinterpret_cast<float4*>(po + i), make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+      if (d0 == 0) __stcg(a.part_ml + (int64_t)pc.slot * kMT + r, make_float2(top, sum));
     }
-  }
-  if (cut && pc.piece == 0 && tid == 0) {
-    Split s = {};
-    s.slot0 = pc.slot;
-    s.pieces = pc.pieces;
-    s.token0 = sq.start;
-    s.rows = nrows;
-    s.head0 = pc.head * a.group;
-    s.row0 = row0;
-    a.splits[pc.split] = s;
-  }
-}
-
-// Joins a cut tile's pieces, one row a CTA: with M = max_s m_s, the output is
-// sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s in piece order. The four warps
-// take every fourth piece each, so that enough loads are in flight for the row
-// to cost one round trip for a few dozen pieces.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a, int rows_most) {
-  constexpr int kV = D / 32, MT = kMT;
-  __shared__ float red[4][D];
-  __shared__ float red_l[4];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nkv = a.l.n_kv_heads;
-  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * rows_most;
-  for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
-    const Split sp = a.splits[x / rows_most];
-    const int r = (int)(x % rows_most);
-    if (r >= sp.rows) continue;  // the same for the whole block
-    auto at = [&](int s) { return ((int64_t)sp.slot0 + (int64_t)s * nkv) * MT + r; };
-    float top = -INFINITY;
-    for (int s = lane; s < sp.pieces; s += 32) top = fmaxf(top, a.part_ml[at(s)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[kV] = {}, sum = 0.f;
-    if (top != -INFINITY) {
+    // (a piece that gave up arrives too, so that the count ends at 0 whatever happens)
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      const int before = atomicAdd(a.arrived + pc.split, 1);
+      last_s = before == pc.pieces - 1;
+      if (last_s) a.arrived[pc.split] = 0;
+      __threadfence();
+    }
+    __syncthreads();
+    if (!last_s) return;
+    // ---- join: warp w takes every fourth piece, four rows at a time, lane l
+    // the outputs from D / 32 * l on; each warp at its own pieces' maximum
+    constexpr int kV = D / 32;
+    const int64_t stride = (int64_t)a.l.n_kv_heads * kMT, first = (int64_t)pc.slot * kMT - pc.piece * stride;
+    const float2* ml = a.part_ml + first + min(lane, kMT - 1);
+    float most = -INFINITY, total = 0.f;
+#pragma unroll 8
+    for (int s = warp; s < pc.pieces; s += kWarps) most = fmaxf(most, __ldcg(ml + s * stride).x);
+#pragma unroll 1
+    for (int q0 = 0; q0 < nrows; q0 += 4) {
+      float part[4][kV] = {};
+      total = 0.f;
 #pragma unroll 4
-      for (int s = warp; s < sp.pieces; s += 4) {
-        const float2 ml = a.part_ml[at(s)];
-        const float f = ex2(ml.x - top);
-        sum += f * ml.y;
-        const float* po = a.part_o + at(s) * D + lane * kV;
-        float v[kV];
-        if constexpr (kV == 4) {
-          const float4 u = *reinterpret_cast<const float4*>(po);
-          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-        } else {
-          const float2 u = *reinterpret_cast<const float2*>(po);
-          v[0] = u.x; v[1] = u.y;
+      for (int s = warp; s < pc.pieces; s += kWarps) {
+        const float2 x = __ldcg(ml + s * stride);
+        const float f = x.x == -INFINITY ? 0.f : ex2(x.x - most);
+        total += f * x.y;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int q = min(q0 + y, nrows - 1);
+          const float fq = __shfl_sync(0xffffffffu, f, q);
+          const float* po = a.part_o + (first + s * stride + q) * D + lane * kV;
+          if constexpr (kV == 4) {
+            const float4 u = __ldcg(reinterpret_cast<const float4*>(po));
+            part[y][0] += fq * u.x;
+            part[y][1] += fq * u.y;
+            part[y][2] += fq * u.z;
+            part[y][3] += fq * u.w;
+          } else {
+            const float2 u = __ldcg(reinterpret_cast<const float2*>(po));
+            part[y][0] += fq * u.x;
+            part[y][1] += fq * u.y;
+          }
         }
-#pragma unroll
-        for (int i = 0; i < kV; ++i) acc[i] += f * v[i];
       }
-    }
 #pragma unroll
-    for (int i = 0; i < kV; ++i) red[warp][lane * kV + i] = acc[i];
-    if (lane == 0) red_l[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x < D / 2) {
-      const int d = 2 * threadIdx.x;
-      const float t = red_l[0] + red_l[1] + red_l[2] + red_l[3], inv = t > 0.f ? 1.0f / t : 0.f;
-      const float lo = (red[0][d] + red[1][d] + red[2][d] + red[3][d]) * inv;
-      const float hi = (red[0][d + 1] + red[1][d + 1] + red[2][d + 1] + red[3][d + 1]) * inv;
-      const int row = sp.row0 + r;
-      T* dst = static_cast<T*>(a.out) + (int64_t)(sp.token0 + row / a.group) * a.ld_out +
-               (int64_t)(sp.head0 + row % a.group) * D + d;
-      *reinterpret_cast<uint32_t*>(dst) = pack2<T>(lo, hi);
+      for (int y = 0; y < 4; ++y)
+        if (q0 + y < nrows)
+#pragma unroll
+          for (int i = 0; i < kV; i += 2)
+            *reinterpret_cast<float2*>(acc + at(q0 + y, lane * kV + i)) = make_float2(part[y][i], part[y][i + 1]);
+    }
+    if (lane < kMT) {
+      sm_m[warp][lane] = most;
+      sm_l[warp][lane] = total;
     }
     __syncthreads();
+    if (r < nrows) add_up();
+    good = true;
+  }
+  if (good && r < nrows) {
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    const int tok = (row0 + r) / a.group;
+    T* dst = static_cast<T*>(a.out) + (int64_t)(sq.start + tok) * a.ld_out +
+             (int64_t)(pc.head * a.group + (row0 + r) % a.group) * D + d0;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 8) {
+      uint4 w;
+      w.x = pack2<T>(v[i] * inv, v[i + 1] * inv);
+      w.y = pack2<T>(v[i + 2] * inv, v[i + 3] * inv);
+      w.z = pack2<T>(v[i + 4] * inv, v[i + 5] * inv);
+      w.w = pack2<T>(v[i + 6] * inv, v[i + 7] * inv);
+      *reinterpret_cast<uint4*>(dst + i) = w;
+    }
   }
 }
-
-int launch_join(ie_dtype dt, int D, Args& a, int rows, int64_t most, cudaStream_t st);
 
 // A page's rows as boxes of 64 dimensions x `box` rows of one head and page,
 // zeros outside. The map lists row and head in the order of their strides.
@@ -561,25 +557,19 @@ int launch_few(Args& a, int64_t grid, cudaStream_t st) {
                 args);
 }
 
-int launch_join(ie_dtype dt, int D, Args& a, int rows, int64_t most, cudaStream_t st) {
-  const int64_t items = most * rows;
-  const unsigned grid = (unsigned)(items < 148 * 8 ? items : 148 * 8);
-  void* args[] = {&a, &rows};
-  auto go = [&](auto kernel) { return launch(kernel, dim3(grid), 128, 0, pdl_launch_enabled(), st, args); };
-  if (dt == IE_DTYPE_F16) return D == 128 ? go(join_kernel<__half, 128>) : go(join_kernel<__half, 64>);
-  return D == 128 ? go(join_kernel<__nv_bfloat16, 128>) : go(join_kernel<__nv_bfloat16, 64>);
-}
-
-// workspace: number of cut tiles | their descriptions | (maximum, sum) | outputs
+// workspace: pieces done of each tile (few rows; zeroed by the caller once) |
+// number of cut tiles | their descriptions (chunks) | (maximum, sum) | outputs
 constexpr int kCapSplits = kTargetFew > kTargetChunk ? kTargetFew : kTargetChunk;
 constexpr int64_t kSlotRowsFew = (int64_t)2 * kTargetFew * kRowsFew;
 constexpr int64_t kSlotRowsChunk = (int64_t)2 * kTargetChunk * kRowsChunk;
 constexpr int64_t kSlotRows = kSlotRowsFew > kSlotRowsChunk ? kSlotRowsFew : kSlotRowsChunk;
-constexpr size_t kOffSplits = 256;
+constexpr size_t kOffCount = 65536;
+static_assert(kCapSplits * sizeof(int) <= kOffCount, "counters");
+constexpr size_t kOffSplits = kOffCount + 64;
 constexpr size_t kOffMl = kOffSplits + kCapSplits * sizeof(Split);
 constexpr size_t kOffO = kOffMl + kSlotRows * sizeof(float2);
 constexpr size_t kWorkspace = kOffO + kSlotRows * 128 * sizeof(float);
-static_assert(kOffMl % 16 == 0 && kOffO % 16 == 0, "alignment of the workspace's parts");
+static_assert(kOffSplits % 16 == 0 && kOffMl % 16 == 0 && kOffO % 16 == 0, "alignment of the workspace's parts");
 
 }  // namespace
 }  // namespace pa
@@ -636,7 +626,6 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   a.scale_log2 = scale * 1.4426950408889634f;
   a.swap_rc = cache->row_stride > cache->head_stride && cache->n_kv_heads > 1;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.n_split = reinterpret_cast<int*>(ws);
   a.splits = reinterpret_cast<Split*>(ws + kOffSplits);
   a.part_ml = reinterpret_cast<float2*>(ws + kOffMl);
   a.part_o = reinterpret_cast<float*>(ws + kOffO);
@@ -649,12 +638,22 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
     const int64_t by_rows = (int64_t)T * group / rows + B;
     return cache->n_kv_heads * (by_seq < by_rows ? by_seq : by_rows);
   };
-  const bool few = (int64_t)max_q * group <= kRowsFew;
+  // Up to 32 rows a sequence and head the few-rows kernel, in one or two tiles:
+  // at 20 and 32 rows it takes 72 us where the chunk kernel takes 85 (32
+  // sequences of 2048 rows) and 117 where that takes 130 (8 of 16384); at 64
+  // rows, in four tiles, 142 against 87.
+  const bool few = (int64_t)max_q * group <= 2 * kRowsFew;
   const int keys = few ? kKB : 64, box = a.l.page_size < keys ? a.l.page_size : keys;
   if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
       !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))
     return IE_ERR_UNSUPPORTED;
   if (!few) {
+    a.n_split = reinterpret_cast<int*>(ws + kOffCount);
+    a.wave = 148;
+    a.whole = 2;
+    a.cut = 6;
+    a.max_pieces = INT_MAX;
+    a.group_magic = 65536 / group + 1;
     a.lane_rows = kRowsChunk / 2 / group * group;
     a.tile_rows = 2 * a.lane_rows;
     a.target = kTargetChunk;
@@ -664,14 +663,18 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
       return IE_ERR_UNSUPPORTED;
     return launch_chunks(dt, D, a, tiles(a.tile_rows), st);
   }
+  a.arrived = reinterpret_cast<int*>(ws);
   a.tile_rows = kRowsFew;
   a.target = kTargetFew;
+  a.wave = 2 * 148;
+  a.whole = 5;
+  a.cut = 9;
   a.min_blocks = 4;
   a.slot_cap = 2 * kTargetFew;
-  const int64_t most = tiles(kRowsFew), grid = most + kTargetFew;
+  const int64_t grid = tiles(kRowsFew) + (B <= 32 ? a.wave : a.target);
   if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
+  a.max_pieces = (int)grid;
   if (dt == IE_DTYPE_F16) s = D == 128 ? launch_few<__half, 128>(a, grid, st) : launch_few<__half, 64>(a, grid, st);
   else s = D == 128 ? launch_few<__nv_bfloat16, 128>(a, grid, st) : launch_few<__nv_bfloat16, 64>(a, grid, st);
-  if (s) return s;
-  return launch_join(dt, D, a, max_q * group, most < kTargetFew ? most : kTargetFew, st);
+  return s;
 }

@@ -34,11 +34,16 @@ struct Args {
   int group, max_q, window, sinks, swap_rc;
   int tile_rows;  // rows of a tile
   int lane_rows;  // chunk kernel: rows of its lane, whole tokens (a tile is two lanes)
+  int group_magic;  // r / group = r * group_magic >> 16 for r < 512
   float scale_log2;
-  int target;     // pieces to aim at
+  int target;     // pieces to aim at in a batch of more than 32 sequences
+  int wave;       // CTAs that run at once
+  int max_pieces; // few rows: CTAs of the launch (a CTA without a piece costs its start)
+  int whole, cut; // start and end of a piece, in blocks
   int min_blocks; // smallest piece
   int slot_cap, split_cap;
-  int* n_split;
+  int* arrived;   // few rows: pieces done of each cut tile, 0 between calls
+  int* n_split;   // chunks: number of cut tiles, and what the joining kernel needs of each
   Split* splits;
   float2* part_ml;  // [slot][row] (maximum in log2 units, sum)
   float* part_o;    // few rows: [slot][16][D]; chunks: [slot][8 warps][D / 4][32 rows][4]
@@ -101,6 +106,13 @@ __device__ __forceinline__ Keys tile_keys(const Args& a, const Seq& s, int tok0,
   k.n_sink = min((k.sink_end + KB - 1) / KB, k.first);
   if (k.n_main == 0) k.n_sink = 0;
   return k;
+}
+
+// Blocks of piece p of P: first and number.
+__device__ __forceinline__ void piece_range(int blocks, int P, int p, int& first, int& n) {
+  const int each = P > 1 ? blocks / P : blocks, more = blocks - each * P;
+  first = p * each + min(p, more);
+  n = each + (p < more);
 }
 
 struct Piece {
@@ -167,15 +179,16 @@ __device__ __forceinline__ Piece piece_at(const Args& a, int b, int tiles, int S
   return p;
 }
 
-// Blocks of a piece for a kernel of one CTA an SM, where whole waves count:
-// lane k - 1 weighs cutting the longest tile into k pieces of C = most / k
-// blocks. With P pieces of A blocks on average, W = ceil(P / SMs) waves cost
-// W (A + o) + C - A blocks, o the start and end of a piece in blocks (about
-// kWhole; kCut with the partial results' way through memory).
-constexpr int kWhole = 5, kCut = 9;
+// Blocks of a piece where whole waves of a.wave CTAs count: lane k - 1 weighs
+// cutting the longest tile into k pieces of C = most / k blocks. With P pieces
+// of A blocks on average, W = ceil(P / wave) waves cost W (A + o) + C - A
+// blocks, o the start and end of a piece in blocks (a.whole; a.cut with the
+// partial results' way through memory). tiles_heads, most: sequence `lane`'s.
 __device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_heads, int most) {
-  const int k = (threadIdx.x & 31) + 1;
-  const int longest = __reduce_max_sync(0xffffffffu, most);
+  const int lane = threadIdx.x & 31;
+  const int longest = __reduce_max_sync(0xffffffffu, most), all = __reduce_add_sync(0xffffffffu, tiles_heads);
+  // (the last lanes: as many pieces as just fill one wave, and two)
+  const int k = lane < 30 ? lane + 1 : max((lane - 29) * a.wave / max(all, 1), 1);
   const int C = max((longest - 1) / k + 1, 1);
   long long pieces = 0, cut = 0, blocks = 0;
   for (int b = 0; b < a.b.B; ++b) {
@@ -186,9 +199,9 @@ __device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_he
     blocks += (long long)t * n;
   }
   const float avg = pieces ? (float)blocks / (float)pieces : 0.f;
-  const float waves = (float)((pieces + a.target - 1) / a.target);
-  float cost = waves * (avg + (cut ? kCut : kWhole)) + (float)C - avg;
-  if (cut > a.slot_cap || (k > 1 && C < a.min_blocks)) cost = INFINITY;
+  const float waves = (float)((pieces + a.wave - 1) / a.wave);
+  float cost = waves * (avg + (cut ? a.cut : a.whole)) + (float)C - avg;
+  if (cut > a.slot_cap || pieces > a.max_pieces || (k > 1 && C < a.min_blocks)) cost = INFINITY;
   float least = cost;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -196,9 +209,112 @@ __device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_he
   return __shfl_sync(0xffffffffu, C, max(who, 0));
 }
 
+// Finds pieces for one warp, in increasing order of their index: sequences are
+// taken 32 at a time, one a lane. The first 32 are read once; the pieces'
+// length comes from the whole batch (by waves for up to 32 sequences).
+template <int KB>
+struct Finder {
+  const Args& a;
+  int C, total, splits;  // blocks of a piece; pieces and cut tiles of the batch
+  int b0;                // first sequence of the held ones
+  Seq s;
+  int tiles, S, mine, x, y, z;  // this lane's; x, y, z inclusive sums of pieces, slots, cut tiles
+  int rx, ry, rz;               // of the sequences before b0
+
+  __device__ __forceinline__ explicit Finder(const Args& args, int* status) : a(args) {
+    const int lane = threadIdx.x & 31;
+    const bool tell = blockIdx.x == 0;
+    if (a.b.B <= 32) {
+      read(0, tell, status);
+      C = piece_blocks_by_waves(a, tiles * a.l.n_kv_heads, most);
+    } else {
+      long long u = 0;
+      for (int b = 0; b < a.b.B; b += 32) {
+        read(b, tell, status);
+        u += (long long)tiles * a.l.n_kv_heads * most;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      C = piece_blocks(a, u);
+    }
+    // the batch's totals: pieces here, cut tiles for the one CTA that reports them
+    rx = ry = rz = 0;
+    if (a.b.B <= 32) {
+      scan();
+    } else {
+      for (int b = 0; b < a.b.B; b += 32) {
+        read(b, false, status);
+        scan();
+        if (b + 32 < a.b.B) skip();
+      }
+    }
+    total = rx + __shfl_sync(0xffffffffu, x, 31);
+    splits = rz + __shfl_sync(0xffffffffu, z, 31);
+    if (a.b.B > 32) {
+      rx = ry = rz = 0;
+      read(0, false, status);
+      scan();
+    }
+    (void)lane;
+  }
+  // Piece `index` (at least the last one asked for); true in the lane that has it.
+  __device__ __forceinline__ bool find(int index, Piece& p, int* status) {
+    while (index >= rx + __shfl_sync(0xffffffffu, x, 31)) {  // index < total
+      skip();
+      read(b0 + 32, false, status);
+      scan();
+    }
+    const int at = index - rx - (x - mine);
+    if (at < 0 || at >= mine) return false;
+    const int nkv = a.l.n_kv_heads;
+    p = piece_at(a, b0 + (threadIdx.x & 31), tiles, S, at, ry + y - (S > 1 ? mine : 0),
+                 rz + z - (S > 1 ? tiles * nkv : 0));
+    return true;
+  }
+
+ private:
+  int most;
+  __device__ __forceinline__ void read(int first, bool tell, int* status) {
+    b0 = first;
+    s = {};
+    tiles = most = 0;
+    const int b = first + (threadIdx.x & 31);
+    if (b < a.b.B) {
+      s = sequence(a, b);
+      tiles = tile_count(a, s);
+      most = most_blocks<KB>(a, s);
+      if (s.bad && tell) atomicExch(status, IE_ERR_INVALID_ARG);
+    }
+  }
+  __device__ __forceinline__ void scan() {
+    const int lane = threadIdx.x & 31, nkv = a.l.n_kv_heads;
+    S = most > C ? (most - 1) / C + 1 : 1;
+    // a count past the range cannot be asked for: the host bounds the pieces
+    mine = (int)min((long long)tiles * S * nkv, 1LL << 25);
+    x = mine;
+    y = S > 1 ? mine : 0;
+    z = S > 1 ? tiles * nkv : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int ux = __shfl_up_sync(0xffffffffu, x, o), uy = __shfl_up_sync(0xffffffffu, y, o),
+                uz = __shfl_up_sync(0xffffffffu, z, o);
+      if (lane >= o) {
+        x += ux;
+        y += uy;
+        z += uz;
+      }
+    }
+  }
+  __device__ __forceinline__ void skip() {
+    rx += __shfl_sync(0xffffffffu, x, 31);
+    ry += __shfl_sync(0xffffffffu, y, 31);
+    rz += __shfl_sync(0xffffffffu, z, 31);
+  }
+};
+
 // The piece a CTA serves and its sequence, in sc; false when there are fewer
-// pieces. Called by the whole block. CTA 0 also writes the number of cut tiles.
-template <int KB, int THREADS, bool kByWaves>
+// pieces. Called by the whole block (few-rows kernel).
+template <int KB, int THREADS>
 __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, int* status) {
   const int tid = threadIdx.x, nkv = a.l.n_kv_heads;
   if (a.b.B <= 32) {
@@ -212,15 +328,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
         most = most_blocks<KB>(a, s);
         if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
       }
-      int C;
-      if constexpr (kByWaves) {
-        C = piece_blocks_by_waves(a, tiles * nkv, most);
-      } else {
-        long long u = (long long)tiles * nkv * most;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-        C = piece_blocks(a, u);
-      }
+      const int C = piece_blocks_by_waves(a, tiles * nkv, most);
       const int S = most > C ? (most - 1) / C + 1 : 1;
       // a count past the grid's range cannot be asked for: the host bounds the pieces
       const int mine = (int)min((long long)tiles * S * nkv, 1LL << 25);
@@ -242,7 +350,6 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
       }
       const unsigned any = __ballot_sync(0xffffffffu, hit);
       if (tid == 0) sc.found = any != 0;
-      if (tid == 31 && index == 0) *a.n_split = min(z, a.split_cap);
     }
     __syncthreads();
     return sc.found != 0;
@@ -289,7 +396,6 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
     for (int j = 0; j < 3; ++j) run[j] += total[j];
     if (index != 0 && run[0] > index) break;
   }
-  if (index == 0 && tid == 0) *a.n_split = run[2] < a.split_cap ? (int)run[2] : a.split_cap;
   __syncthreads();
   return sc.found != 0;
 }
@@ -299,7 +405,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
 int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, cudaStream_t st);
 
 constexpr int kRowsFew = 16;         // tile_rows of the few-rows kernel
-constexpr int kTargetFew = 148 * 8;  // its pieces
+constexpr int kTargetFew = 148 * 4;  // its pieces
 constexpr int kRowsChunk = 256;      // tile_rows of the chunk kernel, at most
 constexpr int kTargetChunk = 148;
 

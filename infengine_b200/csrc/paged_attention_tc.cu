@@ -2,7 +2,7 @@
 // (tcgen05 + TMEM + TMA): the kernel of ie_paged_attention for more rows than
 // the few-rows kernel takes.
 //
-// One CTA serves a piece: up to 256 (token, head) rows of one KV head, as two
+// A piece is up to 256 (token, head) rows of one KV head, as two
 // lanes of up to 128 rows (one TMEM lane a row; whole tokens, so 126 rows in
 // groups of 3), over a range of 64-key blocks. Both lanes use a key or value
 // block from shared memory once it is there, so L2 sees half the traffic of
@@ -30,17 +30,22 @@
 // Operands are 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K
 // K-major, V MN-major as it arrives.
 //
-// Warp roles: 0 copies queries and keys, 2 values (TMA boxes of up to 64 rows
-// of one page; the lanes hold the next table entries), 1 and 3 issue the two
-// lanes' MMAs, 4-7 and 8-11 are the lanes' softmax and epilogue. A barrier wait
-// costs an issuing warp about 110 cycles even when it is over, a TMA or MMA
-// some tens: with one warp for all copies a step of 64 keys took 1900 cycles
-// (2700 with pages of 16), with one for all MMAs 2600. Value rows that no row
-// of the tile sees (range edges inside a block; what the page holds there may
-// be NaN) are zeroed by the MMA warps before the product. Every
-// mbarrier wait is bounded: on expiry IE_ERR_TIMEOUT is recorded, all roles
-// leave their loops, and MMAs and copies in flight are waited for before TMEM
-// is freed.
+// One CTA an SM takes pieces in a back-and-forth order (c, 2G - 1 - c, 2G + c,
+// ..; the longest come first) until none is left, and every role runs ahead
+// of the next as far as its buffers allow: a CTA for each piece spent 10 us of
+// a 30 us piece on finding it, the first copies and the epilogue.
+//
+// Warp roles: 0 finds the pieces and copies queries and keys, 2 values (TMA
+// boxes of up to 64 rows of one page; the lanes hold the next table entries),
+// 1 and 3 issue the two lanes' MMAs, 4-7 and 8-11 are the lanes' softmax and
+// epilogue. A barrier wait costs an issuing warp about 110 cycles even when it
+// is over, a TMA or MMA some tens: with one warp for all copies a step of 64
+// keys took 1900 cycles (2700 with pages of 16), with one for all MMAs 2600.
+// Value rows that no row of the tile sees (range edges inside a block; what the
+// page holds there may be NaN) are zeroed by the MMA warps before the product.
+// Every mbarrier wait is bounded: on expiry IE_ERR_TIMEOUT is recorded, all
+// roles leave their loops, and MMAs and copies in flight are waited for before
+// TMEM is freed.
 #include <cstdio>
 #include <type_traits>
 #include "ie_common.cuh"
@@ -65,19 +70,40 @@ constexpr float kLazy = 8.0f;        // log2 of the growth of a row's maximum th
 
 template <int D>
 struct Cfg {
-  static constexpr int kQTile = 128 * D * 2;                  // a lane's queries
-  static constexpr int kQHalf = 128 * 128;                    // their 64-dimension halves
-  static constexpr int kTile = kKB * D * 2;                   // a key or value block
+  static constexpr int kQTile = 128 * D * 2;      // a lane's queries
+  static constexpr int kQHalf = 128 * 128;        // their 64-dimension halves
+  static constexpr int kTile = kKB * D * 2;       // a key or value block
   static constexpr int kHalf = kKB * 128;
-  static constexpr int kStages = 10;
+  static constexpr int kDepth = 4;                // blocks of keys, and of values, in the ring
+  static constexpr int kOut = 32 * 64 * 2;        // a softmax warp's staging: 32 rows of 64 outputs
   static constexpr int kOffRing = 2 * kQTile;
-  static constexpr int kOffBars = kOffRing + kStages * kTile;
-  static constexpr int kSmem = kOffBars + 512 + 1024;         // + alignment slack
-  // Of 8 pairs of exponentials, those on the FMA pipes. D = 64 has half the
-  // tensor work, so there the special-function unit is the bound.
-  static constexpr int kPoly = 2;
+  static constexpr int kOffOut = kOffRing + 2 * kDepth * kTile;
+  static constexpr int kTiles = kOffOut + 8 * kOut;
+  // Of 8 pairs of exponentials, those on the FMA pipes (0, 2, 3, 4 and 8 took
+  // 1970, 1880, 1830, 1990 and 2590 cycles a step at D = 64).
+  static constexpr int kPoly = 3;
 };
-static_assert(Cfg<128>::kSmem <= 227 * 1024 - 1024, "shared memory per CTA");
+
+// A piece of work, as the roles need it.
+struct Item {
+  int n;                            // blocks; -1: no more pieces
+  int j0;                           // the first of them
+  Keys keys;
+  int seq, head, row_first, tokens; // sequence, KV head, first row of q, tokens of the tile
+  int pos0, rows;                   // position of the first token; rows of the tile
+  int slot, split, piece, pieces;
+};
+
+// What the roles share, before the tiles in shared memory (which begin on a
+// multiple of 1024 bytes).
+struct Control {
+  uint64_t bars[56];
+  Item items[2];
+  int abort, issued[2], queries;
+  uint32_t tmem;
+};
+constexpr int kControl = 1024;
+static_assert(sizeof(Control) <= kControl && kControl + Cfg<128>::kTiles <= 227 * 1024, "shared memory per CTA");
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -221,7 +247,7 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32])
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_wait(bar, parity, abort_flag, &g_paged_tc_status, &g_paged_tc_wait_ns);
 }
 // (the bounded loop stays out of the roles' code, which is long enough to be felt in the instruction cache)
@@ -232,232 +258,323 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Args a) {
   using C = Cfg<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
-  __shared__ Scan scan;
-  __shared__ uint32_t tmem_holder;
-  __shared__ int abort_s, issued_s[2];
-  volatile int* abort_flag = &abort_s;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Control& ctl = *reinterpret_cast<Control*>(smem_raw);
+  uint8_t* smem = smem_raw + kControl;
+  volatile int* abort_flag = &ctl.abort;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  auto full_bar = [&](int s) { return smem_u32(bars + s); };
-  auto empty_bar = [&](int s) { return smem_u32(bars + C::kStages + s); };
-  constexpr int kB = 2 * C::kStages;
-  const uint32_t q_full = smem_u32(bars + kB);
-  auto s_full = [&](int i, int b) { return smem_u32(bars + kB + 1 + 2 * i + b); };  // scores of lane i, buffer b
-  auto p_full = [&](int i, int b) { return smem_u32(bars + kB + 5 + 2 * i + b); };
-  auto pv_done = [&](int i) { return smem_u32(bars + kB + 9 + i); };
-  auto o_full = [&](int i) { return smem_u32(bars + kB + 11 + i); };
-  auto drain_bar = [&](int i) { return smem_u32(bars + kB + 13 + i); };
-  static_assert((kB + 15) * 8 <= 512, "barriers");
+  constexpr int kDepth = C::kDepth;
+  const uint32_t bars = smem_u32(ctl.bars);
+  auto full_bar = [&](int s) { return bars + 8 * s; };                     // keys 0 .., values kDepth ..
+  auto empty_bar = [&](int s) { return bars + 8 * (2 * kDepth + s); };
+  constexpr int kB = 4 * kDepth;
+  const uint32_t q_full = bars + 8 * kB, q_empty = bars + 8 * (kB + 1);
+  auto item_full = [&](int t) { return bars + 8 * (kB + 2 + (t & 1)); };
+  auto item_empty = [&](int t) { return bars + 8 * (kB + 4 + (t & 1)); };
+  auto s_full = [&](int i, int b) { return bars + 8 * (kB + 6 + 2 * i + b); };  // scores of lane i, buffer b
+  auto p_full = [&](int i, int b) { return bars + 8 * (kB + 10 + 2 * i + b); };
+  // by buffer too: two products may be done before the issuing warp asks for the first
+  auto pv_done = [&](int i, int b) { return bars + 8 * (kB + 14 + 2 * i + b); };
+  auto o_full = [&](int i) { return bars + 8 * (kB + 18 + i); };
+  auto o_empty = [&](int i) { return bars + 8 * (kB + 20 + i); };
+  auto drain_bar = [&](int i) { return bars + 8 * (kB + 22 + i); };
+  static_assert(kB + 24 <= 56, "barriers");
 
   if (threadIdx.x == 32) {
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < 2 * kDepth; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 2);  // both lanes' MMAs
     }
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(pv_done(i), 1);
+      mbar_init(item_full(i), 1);
+      mbar_init(item_empty(i), 11);  // every warp but the finding one
       mbar_init(o_full(i), 1);
+      mbar_init(o_empty(i), 4);
       mbar_init(drain_bar(i), 1);
       for (int b = 0; b < 2; ++b) {
         mbar_init(s_full(i, b), 1);
+        mbar_init(pv_done(i, b), 1);
         mbar_init(p_full(i, b), 4);
       }
     }
-    abort_s = 0;
-    issued_s[0] = issued_s[1] = 0;
+    ctl.abort = 0;
+    ctl.issued[0] = ctl.issued[1] = ctl.queries = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&a.tmQ);
     prefetch_map(&a.tmK);
     prefetch_map(&a.tmV);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (!find_piece<kKB, kThreads, true>(a, blockIdx.x, scan, &g_paged_tc_status)) return;
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)),
                  "n"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_holder;
+  const uint32_t tmem = ctl.tmem;
 
-  const Piece pc = scan.p;
-  const Seq sq = scan.seq;
-  const int row0 = pc.tile * a.tile_rows, nrows = min(a.tile_rows, sq.tokens * a.group - row0);
-  const int tok0 = row0 / a.group, tok1 = tok0 + (nrows - 1) / a.group;
-  const Keys ks = tile_keys<kKB>(a, sq, tok0, tok1);
-  const int all = ks.blocks();
-  const int j0 = (int)((int64_t)all * pc.piece / pc.pieces);
-  const int n = (int)((int64_t)all * (pc.piece + 1) / pc.pieces) - j0;  // blocks of this piece
-  const bool two = nrows > a.lane_rows;
-  // stage and phase of block j's keys (v = 0) or values (1): each has half the ring
-  constexpr int kDepth = C::kStages / 2;
-  auto stage = [&](int v, int j) { return v * kDepth + j % kDepth; };
-  auto phase = [&](int j) { return (uint32_t)((j / kDepth) & 1); };
+  // Blocks are counted over all pieces, by the copies and by each lane: block
+  // g of the copies lies in stage g % kDepth, scores of block g of a lane in
+  // buffer g & 1.
+  auto phase = [&](int g) { return (uint32_t)((g / kDepth) & 1); };
+  auto over = [&](uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait(bar, parity, abort_flag)) != 0;
+  };
+  // piece t's description; the slot is free for the next but one once every warp has its copy
+  auto take = [&](int t, Item& it) {
+    if (!over(item_full(t), (uint32_t)((t >> 1) & 1))) return false;
+    it = ctl.items[t & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty(t));
+    return it.n >= 0;
+  };
 
-  if (warp == 0 || warp == 2) {
-    // ------------------------------------------------ copies of keys (0) or values (2)
-    const int v = warp >> 1;
-    const int nu = __shfl_sync(0xffffffffu, n, 0), head = __shfl_sync(0xffffffffu, pc.head, 0);
-    const CUtensorMap* map = v ? &a.tmV : &a.tmK;
-    if (v == 0 && nu > 0 && elect_one()) {
-      mbar_expect_tx(q_full, (two ? 2 : 1) * a.lane_rows * D * 2);
-      for (int i = 0; i < (two ? 2 : 1); ++i)
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          tma_load_3d(smem_u32(smem + i * C::kQTile + h * C::kQHalf), &a.tmQ, q_full, 64 * h, head * a.group,
-                      sq.start + tok0 + i * (a.lane_rows / a.group));
-    }
-    // rows of a copy, copies of a block's half, blocks whose table entries the warp holds
-    const int box_log2 = min(a.l.page_log2, 6), box = 1 << box_log2, boxes_log2 = 6 - box_log2;
-    const int held_log2 = 5 - boxes_log2;
-    const int* table = a.b.page_table + (int64_t)pc.b * a.b.ld_table;
-    auto load_entries = [&](int it0) {
-      const int it = it0 + (lane >> boxes_log2);
-      if (it >= n) return -1;
-      const int kb = ks.block(j0 + it) * kKB + (lane & ((1 << boxes_log2) - 1)) * box;
-      if (!(kb < ks.hi && (kb + box > ks.lo || kb < ks.sink_end))) return -1;
-      const int page = table[kb >> a.l.page_log2];
-      if (page < 0 || page >= a.l.num_pages) {
-        atomicExch(&g_paged_tc_status, IE_ERR_INVALID_ARG);
-        return a.l.num_pages;  // outside the tensor map: zeros
-      }
-      return page;
-    };
-    int entries = load_entries(0), next = load_entries(1 << held_log2), issued = 0;
-    for (int j = 0; j < nu; ++j) {
-      const int at = j & ((1 << held_log2) - 1);
-      if (j > 0 && at == 0) {
-        entries = next;
-        next = load_entries(j + (1 << held_log2));
-      }
-      const uint32_t full = full_bar(stage(v, j)), dst = smem_u32(smem + C::kOffRing + stage(v, j) * C::kTile);
-      const int r0 = (ks.block(j0 + j) * kKB) & (a.l.page_size - 1);
-      int page[4], copies = 0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        page[x] = __shfl_sync(0xffffffffu, entries, ((at << boxes_log2) + x) & 31);
-        if (x >> boxes_log2) page[x] = -1;
-        copies += page[x] >= 0;
-      }
-      if (!__all_sync(0xffffffffu, wait(empty_bar(stage(v, j)), phase(j) ^ 1u, abort_flag))) break;
-      if (elect_one()) {
-        mbar_expect_tx(full, copies * box * D * 2);
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (page[x] >= 0) {
-            const int r = (r0 + x * box) & (a.l.page_size - 1);
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h)
-              tma_load_4d(dst + h * C::kHalf + x * box * 128, map, full, 64 * h, a.swap_rc ? head : r,
-                          a.swap_rc ? r : head, page[x]);
+  // Registers: 384 x 168 at launch; the softmax warps take 216 each, the
+  // others give up down to 72.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0 || warp == 2) {
+      // ---------------------------------------------- copies of queries and keys (0) or values (2)
+      const int v = warp >> 1;
+      const CUtensorMap* map = v ? &a.tmV : &a.tmK;
+      // rows of a copy, copies of a block's half, blocks whose table entries the warp holds
+      const int box_log2 = min(a.l.page_log2, 6), box = 1 << box_log2, boxes_log2 = 6 - box_log2;
+      const int held_log2 = 5 - boxes_log2, held = 1 << held_log2;
+      int g = 0, queries = 0;  // blocks and query tiles copied so far
+      // the copies of one piece; false when a wait gave up
+      auto copy = [&](const Item& it) {
+        const int n = __shfl_sync(0xffffffffu, it.n, 0), head = __shfl_sync(0xffffffffu, it.head, 0);
+        if (n == 0) return true;
+        const bool two = it.rows > a.lane_rows;
+        const int* table = a.b.page_table + (int64_t)it.seq * a.b.ld_table;
+        auto load_entries = [&](int first) {
+          const int j = first + (lane >> boxes_log2);
+          if (j >= n) return -1;
+          const int kb = it.keys.block(it.j0 + j) * kKB + (lane & ((1 << boxes_log2) - 1)) * box;
+          if (!(kb < it.keys.hi && (kb + box > it.keys.lo || kb < it.keys.sink_end))) return -1;
+          const int page = table[kb >> a.l.page_log2];
+          if (page < 0 || page >= a.l.num_pages) {
+            atomicExch(&g_paged_tc_status, IE_ERR_INVALID_ARG);
+            return a.l.num_pages;  // outside the tensor map: zeros
           }
+          return page;
+        };
+        int entries = load_entries(0), next = load_entries(held);
+        if (v == 0) {
+          // the last piece's scores are done with its queries
+          if (!over(q_empty, (uint32_t)((queries & 1) ^ 1))) return false;
+          if (elect_one()) {
+            mbar_expect_tx(q_full, (two ? 2 : 1) * a.lane_rows * D * 2);
+            for (int i = 0; i < (two ? 2 : 1); ++i)
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+                tma_load_3d(smem_u32(smem + i * C::kQTile + h * C::kQHalf), &a.tmQ, q_full, 64 * h, head * a.group,
+                            it.row_first + i * (a.lane_rows / a.group));
+          }
+          ++queries;
+        }
+        for (int j = 0; j < n; ++j, ++g) {
+          const int at = j & (held - 1);
+          if (j > 0 && at == 0) {
+            entries = next;
+            next = load_entries(j + held);
+          }
+          const int s = v * kDepth + g % kDepth;
+          const uint32_t full = full_bar(s), dst = smem_u32(smem + C::kOffRing + s * C::kTile);
+          const int r0 = (it.keys.block(it.j0 + j) * kKB) & (a.l.page_size - 1);
+          int page[4], copies = 0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            page[x] = __shfl_sync(0xffffffffu, entries, ((at << boxes_log2) + x) & 31);
+            if (x >> boxes_log2) page[x] = -1;
+            copies += page[x] >= 0;
+          }
+          if (!over(empty_bar(s), phase(g) ^ 1u)) return false;
+          if (elect_one()) {
+            mbar_expect_tx(full, copies * box * D * 2);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (page[x] >= 0) {
+                const int r = (r0 + x * box) & (a.l.page_size - 1);
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h)
+                  tma_load_4d(dst + h * C::kHalf + x * box * 128, map, full, 64 * h, a.swap_rc ? head : r,
+                              a.swap_rc ? r : head, page[x]);
+              }
+          }
+        }
+        return true;
+      };
+      Item it;
+      if (v == 1) {
+        for (int t = 0; take(t, it) && copy(it); ++t) {
+        }
+      } else {
+        Finder<kKB> finder(a, &g_paged_tc_status);
+        if (blockIdx.x == 0 && lane == 0) *a.n_split = min(finder.splits, a.split_cap);
+        const int G = gridDim.x, c = blockIdx.x;
+        for (int t = 0;; ++t) {
+          if (!over(item_empty(t), (uint32_t)(((t >> 1) & 1) ^ 1))) break;
+          const int index = t * G + ((t & 1) ? G - 1 - c : c);
+          const bool more = index < finder.total;
+          if (more) {
+            Piece p;
+            if (finder.find(index, p, &g_paged_tc_status)) {
+              const Seq& sq = finder.s;
+              const int row0 = p.tile * a.tile_rows, per = a.tile_rows / a.group, tok0 = p.tile * per;
+              Item x;
+              x.rows = min(a.tile_rows, sq.tokens * a.group - row0);
+              x.tokens = min(per, sq.tokens - tok0);
+              x.keys = tile_keys<kKB>(a, sq, tok0, tok0 + x.tokens - 1);
+              piece_range(x.keys.blocks(), p.pieces, p.piece, x.j0, x.n);
+              x.seq = p.b;
+              x.head = p.head;
+              x.row_first = sq.start + tok0;
+              x.pos0 = sq.pos0 + tok0;
+              x.slot = p.slot;
+              x.split = p.split;
+              x.piece = p.piece;
+              x.pieces = p.pieces;
+              ctl.items[t & 1] = x;
+            }
+          } else if (lane == 0) {
+            ctl.items[t & 1].n = -1;
+          }
+          __syncwarp();
+          it = ctl.items[t & 1];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(item_full(t));
+          if (!more || !copy(it)) break;
+        }
+        if (lane == 0) ctl.queries = queries;
       }
-      issued = j + 1;
-    }
-    if (lane == 0) issued_s[v] = issued;
-  } else if (warp == 1 || warp == 3) {
-    const int i = warp >> 1;
-    if (n > 0 && (i == 0 || two)) {
+      if (lane == 0) ctl.issued[v] = g;
+    } else {
       // ---------------------------------------------- MMAs of lane i
+      const int i = warp >> 1;
       const uint32_t id_qk = idesc_f16<T>(128, kKB, 0), id_pv = idesc_f16<T>(128, D, 1);
       const uint32_t ring = smem_u32(smem + C::kOffRing);
       const uint64_t qs = sw128_desc(smem_u32(smem) + i * C::kQTile);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + 128 * i;
-      const int nu = __shfl_sync(0xffffffffu, n, 0);
-      const bool alone = __shfl_sync(0xffffffffu, (int)two, 0) == 0;
-      auto over = [&](uint32_t bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, wait(bar, parity, abort_flag)) != 0;
-      };
-      // the stage is free when both lanes' MMAs so far are done
-      auto release = [&](int s) {
-        mma_commit(empty_bar(s));
-        if (alone) mma_commit(empty_bar(s));
-      };
-      auto qk = [&](int j) {  // scores of block j
-        const int s = stage(0, j);
-        if (!over(full_bar(s), phase(j))) return false;
-        fence_after();
-        const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_f16(tm + 64 * (j & 1), qs + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
-                    sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
-          mma_commit(s_full(i, j & 1));
-          release(s);
+      int gc = 0, g = 0, tiles = 0, queries = 0;  // blocks of the copies and of this lane, its tiles, query tiles
+      Item it;
+      bool ok = true;
+      for (int t = 0; ok && take(t, it); ++t) {
+        const int n = __shfl_sync(0xffffffffu, it.n, 0);
+        if (n == 0) continue;
+        const bool two = __shfl_sync(0xffffffffu, it.rows, 0) > a.lane_rows;
+        if (i == 1 && !two) {
+          // nothing for this lane: it only passes everything on (no phase may
+          // go by unseen, the next wait could not tell it from its own)
+          ok = over(q_full, (uint32_t)(queries++ & 1));
+          if (ok && lane == 0) mbar_arrive(q_empty);
+          for (int j = 0; ok && j < n; ++j, ++gc)
+            for (int v = 0; ok && v < 2; ++v) {
+              const int s = v * kDepth + gc % kDepth;
+              ok = over(full_bar(s), phase(gc));
+              if (ok && lane == 0) mbar_arrive(empty_bar(s));
+            }
+          continue;
         }
-        return true;
-      };
-      bool ok = over(q_full, 0);
-      for (int j = 0; ok && j < min(nu, 2); ++j) ok = qk(j);
-      for (int j = 0; ok && j < nu; ++j) {
-        const int s = stage(1, j), kb = ks.block(j0 + j) * kKB;
-        if (!(ok = over(full_bar(s), phase(j)))) break;
-        if (kb + kKB > ks.hi || (kb < ks.lo && kb + kKB > ks.sink_end)) {
-          // rows that no row of the tile sees (both lanes' warps write the same zeros)
-          uint8_t* v = smem + C::kOffRing + s * C::kTile;
-          for (int r = lane; r < kKB; r += 32) {
-            const int key = kb + r;
-            if (!(key < ks.hi && (key >= ks.lo || key < ks.sink_end)))
+        auto qk = [&](int j) {  // scores of block j, into the buffer of block g + j - 2
+          const int s = (gc + j) % kDepth, b = (g + j) & 1;
+          if (g + j >= 2 && !over(pv_done(i, b), (uint32_t)(((g + j - 2) >> 1) & 1))) return false;
+          if (!over(full_bar(s), phase(gc + j))) return false;
+          fence_after();
+          const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
+          if (elect_one()) {
 #pragma unroll
-              for (int c = 0; c < D / 8; ++c)
-                *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < D / 16; ++k)
+              mma_f16(tm + 64 * b, qs + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
+                      sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
+            mma_commit(s_full(i, b));
+            mma_commit(empty_bar(s));
+            if (j == n - 1) mma_commit(q_empty);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        if (!(ok = over(p_full(i, j & 1), (uint32_t)((j >> 1) & 1)))) break;
-        fence_after();
-        const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
-        if (elect_one()) {
+          return true;
+        };
+        ok = over(q_full, (uint32_t)(queries & 1));
+        ++queries;
+        for (int j = 0; ok && j < min(n, 2); ++j) ok = qk(j);
+        // the epilogue has read the last tile's outputs
+        if (ok && tiles > 0) ok = over(o_empty(i), (uint32_t)((tiles - 1) & 1));
+        for (int j = 0; ok && j < n; ++j) {
+          const int s = kDepth + (gc + j) % kDepth, kb = it.keys.block(it.j0 + j) * kKB, b = (g + j) & 1;
+          if (!(ok = over(full_bar(s), phase(gc + j)))) break;
+          if (kb + kKB > it.keys.hi || (kb < it.keys.lo && kb + kKB > it.keys.sink_end)) {
+            // rows that no row of the tile sees (both lanes' warps write the same zeros)
+            uint8_t* v = smem + C::kOffRing + s * C::kTile;
+            for (int r = lane; r < kKB; r += 32) {
+              const int key = kb + r;
+              if (!(key < it.keys.hi && (key >= it.keys.lo || key < it.keys.sink_end)))
 #pragma unroll
-          for (int k = 0; k < kKB / 16; ++k)
-            mma_ts(tm + 256, tm + 64 * (j & 1) + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
-          mma_commit(pv_done(i));
-          if (j == nu - 1) mma_commit(o_full(i));
-          release(s);
+                for (int c = 0; c < D / 8; ++c)
+                  *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) =
+                      make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          if (!(ok = over(p_full(i, b), (uint32_t)(((g + j) >> 1) & 1)))) break;
+          fence_after();
+          const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kKB / 16; ++k)
+              mma_ts(tm + 256, tm + 64 * b + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
+            mma_commit(pv_done(i, b));
+            if (j == n - 1) mma_commit(o_full(i));
+            mma_commit(empty_bar(s));
+          }
+          // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
+          if (j + 2 < n) ok = qk(j + 2);
         }
-        // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
-        if (j + 2 < nu) ok = over(pv_done(i), (uint32_t)(j & 1)) && qk(j + 2);
+        gc += n;
+        g += n;
+        ++tiles;
       }
-      if (*abort_flag) {
-        // every MMA issued so far is done before TMEM is released
-        __syncwarp();
-        if (elect_one()) mma_commit(drain_bar(i));
-        const unsigned long long t0 = globaltimer();
-        while (!mbar_try(drain_bar(i), 0) && globaltimer() - t0 < kDrainWaitNs) {
-        }
+      // every MMA issued is done before TMEM is released, whoever gave up
+      __syncwarp();
+      if (elect_one()) mma_commit(drain_bar(i));
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try(drain_bar(i), 0) && globaltimer() - t0 < kDrainWaitNs) {
       }
     }
     __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------ softmax and epilogue
     const int i = (warp - 4) >> 2, quad = warp & 3;  // TMEM lane quarter = warp & 3
     const int r = 32 * quad + lane;                  // row of the lane
     const int row = r < a.lane_rows ? i * a.lane_rows + r : INT_MAX;  // row of the tile
     const uint32_t tl = (uint32_t)(32 * quad) << 16;
     const uint32_t to = tmem + tl + 256 + 128 * i;
-    const int last = min(nrows, (i + 1) * a.lane_rows) - 1;  // the lane's last row
-    const int pos = row < nrows ? sq.pos0 + tok0 + row / a.group : -1;
-    const int pos_min = sq.pos0 + tok0 + i * a.lane_rows / a.group, pos_max = sq.pos0 + tok0 + last / a.group;
     // a scale of 0 weighs all seen keys alike: scores 0, so that masked ones can stay infinite
     const bool flat = a.scale_log2 == 0.f;
     const float c = flat ? 1.0f : a.scale_log2;
-    float m = -INFINITY, l = 0.f;  // m: the reference, in log2 units
+    const int my_token = row < INT_MAX ? row * a.group_magic >> 16 : 0;
+    int g = 0, tiles = 0;  // this lane's blocks and tiles so far
+    Item it;
     bool ok = true;
-    if (i == 0 || two) {
+    for (int t = 0; ok && take(t, it); ++t) {
+      if (i == 1 && it.rows <= a.lane_rows) continue;
+      const int n = it.n;
+      const bool valid = row < it.rows;
+      const int pos = valid ? it.pos0 + my_token : -1;
+      const int pos_min = it.pos0 + i * (a.lane_rows / a.group);
+      const int pos_max = it.pos0 + min(it.tokens, (i + 1) * (a.lane_rows / a.group)) - 1;
+      float m = -INFINITY, l = 0.f;  // m: the reference, in log2 units
       for (int j = 0; j < n; ++j) {
-        const int kb = ks.block(j0 + j) * kKB;
-        const uint32_t ts = tmem + tl + 128 * i + 64 * (j & 1);
-        ok = __all_sync(0xffffffffu, wait(s_full(i, j & 1), (uint32_t)((j >> 1) & 1), abort_flag));
+        const int kb = it.keys.block(it.j0 + j) * kKB, b = (g + j) & 1;
+        const uint32_t ts = tmem + tl + 128 * i + 64 * b;
+        ok = over(s_full(i, b), (uint32_t)(((g + j) >> 1) & 1));
         if (!ok) break;
         fence_after();
         float v[kKB];
@@ -489,16 +606,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         float top;
         {
           if (c > 0.f) {
-            float t[4];
+            float t4[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) t[x] = v[x];
+            for (int x = 0; x < 4; ++x) t4[x] = v[x];
 #pragma unroll
             for (int x = 4; x + 8 <= kKB; x += 8)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) t[y] = max3(t[y], v[x + 2 * y], v[x + 2 * y + 1]);
+              for (int y = 0; y < 4; ++y) t4[y] = max3(t4[y], v[x + 2 * y], v[x + 2 * y + 1]);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) t[y] = max3(t[y], v[kKB - 4 + 2 * y], v[kKB - 3 + 2 * y]);
-            top = max3(max3(t[0], t[1], t[2]), t[3], t[3]) * c;
+            for (int y = 0; y < 2; ++y) t4[y] = max3(t4[y], v[kKB - 4 + 2 * y], v[kKB - 3 + 2 * y]);
+            top = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * c;
           } else {
             top = v[0] * c;
 #pragma unroll
@@ -506,13 +623,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
         }
         // (a NaN or infinite score turns the row's reference, and with it the row, into NaN)
-        const bool rise = row < nrows && !(top <= m + kLazy);
+        const bool rise = valid && !(top <= m + kLazy);
         if (__any_sync(0xffffffffu, rise)) {
           const float to_m = !rise ? m : top < INFINITY ? top : __int_as_float(0x7fffffff);
           const float f = rise ? ex2(m - to_m) : 1.0f;
           if (j > 0) {
             // every product before this block's
-            ok = __all_sync(0xffffffffu, wait(pv_done(i), (uint32_t)((j - 1) & 1), abort_flag));
+            ok = over(pv_done(i, b ^ 1), (uint32_t)(((g + j - 1) >> 1) & 1));
             if (!ok) break;
             fence_after();
 #pragma unroll
@@ -559,77 +676,88 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         tmem_st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(i, j & 1));
+        if (lane == 0) mbar_arrive(p_full(i, b));
       }
-    }
-    // ---- epilogue
-    const bool cut = pc.slot >= 0;
-    if (i == 0 || two) {
-      // (a barrier of its own: two products may be done since this warp last looked at pv_done)
-      if (ok && n > 0) ok = wait(o_full(i), 0, abort_flag);
-      ok = __all_sync(0xffffffffu, ok) && (!cut || (pc.slot < a.slot_cap && pc.split < a.split_cap));
+      // ---- epilogue
+      if (ok && n > 0) ok = over(o_full(i), (uint32_t)(tiles & 1));
+      if (!ok) break;
       fence_after();
-      if (ok && cut) {
+      const bool cut = it.slot >= 0;
+      if (cut && (it.slot >= a.slot_cap || it.split >= a.split_cap)) {
+        // cannot be: the pieces were chosen to fit
+      } else if (cut) {
         // row-interleaved 16-byte pieces, so that a warp's stores are contiguous
-        float4* po = reinterpret_cast<float4*>(a.part_o) + ((int64_t)pc.slot * 8 + 4 * i + quad) * (D / 4) * 32 + lane;
+        float4* po =
+            reinterpret_cast<float4*>(a.part_o) + ((int64_t)it.slot * 8 + 4 * i + quad) * (D / 4) * 32 + lane;
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
-          uint32_t w[32] = {};
-          if (n > 0) {
-            tmem_ld(to + 32 * x, w);
-            tmem_ld_wait(w);
+          uint32_t w[32];
+          tmem_ld(to + 32 * x, w);
+          tmem_ld_wait(w);
+          if (n == 0) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) w[y] = 0u;
           }
 #pragma unroll
           for (int y = 0; y < 8; ++y)
             po[(8 * x + y) * 32] = make_float4(__uint_as_float(w[4 * y]), __uint_as_float(w[4 * y + 1]),
                                                __uint_as_float(w[4 * y + 2]), __uint_as_float(w[4 * y + 3]));
         }
-        a.part_ml[(int64_t)pc.slot * kRowsChunk + 128 * i + r] = make_float2(m, l);
-        if (pc.piece == 0 && i == 0 && r == 0) {
+        a.part_ml[(int64_t)it.slot * kRowsChunk + 128 * i + r] = make_float2(m, l);
+        if (it.piece == 0 && i == 0 && r == 0) {
           Split sp = {};
-          sp.slot0 = pc.slot;
-          sp.pieces = pc.pieces;
-          sp.token0 = sq.start + tok0;
-          sp.rows = nrows;
-          sp.head0 = pc.head * a.group;
-          a.splits[pc.split] = sp;
+          sp.slot0 = it.slot;
+          sp.pieces = it.pieces;
+          sp.token0 = it.row_first;
+          sp.rows = it.rows;
+          sp.head0 = it.head * a.group;
+          a.splits[it.split] = sp;
         }
-      } else if (ok) {
-        // through the lane's Q tile (its products are done): swizzled rows in,
-        // D / 8 lanes a row out
+      } else {
+        // through the warp's staging, 64 outputs at a time: swizzled rows in, 8 lanes a row out
         const float inv = l > 0.f ? 1.0f / l : 0.f;
-        uint8_t* st = smem + i * C::kQTile + 32 * quad * D * 2;
+        uint8_t* st = smem + C::kOffOut + (4 * i + quad) * C::kOut;
+#pragma unroll 1
+        for (int h = 0; h < D / 64; ++h) {
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          uint32_t w[32] = {};
-          if (n > 0) {
-            tmem_ld(to + 32 * x, w);
+          for (int z = 0; z < 2; ++z) {
+            uint32_t w[32];
+            tmem_ld(to + 64 * h + 32 * z, w);
             tmem_ld_wait(w);
-          }
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            uint4 u;
-            u.x = pack2<T>(__uint_as_float(w[8 * y]) * inv, __uint_as_float(w[8 * y + 1]) * inv);
-            u.y = pack2<T>(__uint_as_float(w[8 * y + 2]) * inv, __uint_as_float(w[8 * y + 3]) * inv);
-            u.z = pack2<T>(__uint_as_float(w[8 * y + 4]) * inv, __uint_as_float(w[8 * y + 5]) * inv);
-            u.w = pack2<T>(__uint_as_float(w[8 * y + 6]) * inv, __uint_as_float(w[8 * y + 7]) * inv);
-            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * x + y) ^ (lane & 7)) << 4)) = u;
+            for (int y = 0; y < 4; ++y) {
+              uint4 u = make_uint4(0, 0, 0, 0);
+              if (n > 0) {
+                u.x = pack2<T>(__uint_as_float(w[8 * y]) * inv, __uint_as_float(w[8 * y + 1]) * inv);
+                u.y = pack2<T>(__uint_as_float(w[8 * y + 2]) * inv, __uint_as_float(w[8 * y + 3]) * inv);
+                u.z = pack2<T>(__uint_as_float(w[8 * y + 4]) * inv, __uint_as_float(w[8 * y + 5]) * inv);
+                u.w = pack2<T>(__uint_as_float(w[8 * y + 6]) * inv, __uint_as_float(w[8 * y + 7]) * inv);
+              }
+              *reinterpret_cast<uint4*>(st + lane * 128 + (((4 * z + y) ^ (lane & 7)) << 4)) = u;
+            }
           }
+          __syncwarp();
+          T* out = static_cast<T*>(a.out) + (int64_t)it.row_first * a.ld_out + (int64_t)it.head * a.group * D +
+                   64 * h + 8 * (lane & 7);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int q = 4 * x + (lane >> 3), rr = 32 * quad + q, gr = i * a.lane_rows + rr;
+            if (rr < a.lane_rows && gr < it.rows) {
+              const int tok = gr * a.group_magic >> 16;
+              *reinterpret_cast<uint4*>(out + (int64_t)tok * a.ld_out + (gr - tok * a.group) * D) =
+                  *reinterpret_cast<const uint4*>(st + q * 128 + (((lane & 7) ^ (q & 7)) << 4));
+            }
+          }
+          __syncwarp();
         }
+      }
+      if (n > 0) {
+        // the outputs are read: the next tile's first product may overwrite them
+        fence_before();
         __syncwarp();
-        constexpr int kChunks = D / 8, kRows = 32 / kChunks;
-        const int cc = lane % kChunks;
-        T* out = static_cast<T*>(a.out) + (int64_t)(sq.start + tok0) * a.ld_out + (int64_t)pc.head * a.group * D +
-                 8 * cc;
-#pragma unroll 4
-        for (int x = 0; x < 32 / kRows; ++x) {
-          const int q = x * kRows + lane / kChunks, rr = 32 * quad + q, g = i * a.lane_rows + rr;
-          if (rr < a.lane_rows && g < nrows) {
-            const int tok = g / a.group;
-            *reinterpret_cast<uint4*>(out + (int64_t)tok * a.ld_out + (g - tok * a.group) * D) =
-                *reinterpret_cast<const uint4*>(st + q * D * 2 + ((cc ^ (q & 7)) << 4));
-          }
-        }
+        if (lane == 0) mbar_arrive(o_empty(i));
+        ++tiles;
+        g += n;
       }
     }
   }
@@ -639,16 +767,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __syncthreads();
   fence_after();
   if (*abort_flag && threadIdx.x == 0) {
-    // copies still in flight land before the CTA exits: the queries, and the
-    // last kDepth blocks of keys and values (an earlier one's stage was reused)
+    // copies still in flight land before the CTA exits: the last queries, and
+    // the last kDepth blocks of keys and values (an earlier one's stage was reused)
     auto landed = [&](uint32_t bar, uint32_t parity) {
       const unsigned long long t0 = globaltimer();
       while (!mbar_try(bar, parity) && globaltimer() - t0 < kDrainWaitNs / 4) {
       }
     };
-    if (n > 0) landed(q_full, 0);
+    if (ctl.queries > 0) landed(q_full, (uint32_t)((ctl.queries - 1) & 1));
     for (int v = 0; v < 2; ++v)
-      for (int j = max(0, issued_s[v] - kDepth); j < issued_s[v]; ++j) landed(full_bar(stage(v, j)), phase(j));
+      for (int g = max(0, ctl.issued[v] - kDepth); g < ctl.issued[v]; ++g)
+        landed(full_bar(v * kDepth + g % kDepth), phase(g));
   }
   __syncthreads();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
@@ -718,13 +847,14 @@ int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return IE_ERR_LAUNCH;
   static bool configured[64] = {};
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kControl + Cfg<D>::kTiles) !=
+        cudaSuccess)
       return IE_ERR_LAUNCH;
     configured[dev] = true;
   }
-  const int64_t grid = most_tiles + a.slot_cap;
-  if (grid > INT_MAX) return IE_ERR_UNSUPPORTED;
-  kernel<<<(unsigned)grid, kThreads, Cfg<D>::kSmem, st>>>(a);
+  if (most_tiles + a.slot_cap > INT_MAX) return IE_ERR_UNSUPPORTED;
+  const int64_t most = most_tiles + a.slot_cap, grid = most < a.wave ? most : a.wave;
+  kernel<<<(unsigned)grid, kThreads, kControl + Cfg<D>::kTiles, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) {
     const int64_t items = 8 * (most_tiles < a.target ? most_tiles : a.target);

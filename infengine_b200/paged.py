@@ -105,8 +105,10 @@ def paged_attention_workspace_bytes() -> int:
 
 
 def paged_attention_workspace(device="cuda"):
-    """A workspace for paged_attention; it needs no initialisation."""
-    return torch.empty(paged_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+    """A workspace for paged_attention, its counters zeroed."""
+    ws = torch.empty(paged_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+    ws[:65536].zero_()
+    return ws
 
 
 def paged_attention(q, cache, page_table, q_start, kv_len, out, max_q, window=0, sinks=0, scale=None, workspace=None,

@@ -14,10 +14,11 @@ def run_attention(ie, cuda, s, window=0, sinks=0, scale=None, out=None, max_q=No
         out = cuda.full((T, s["heads"] * s["dim"]), 77.0, dtype=s["q"].dtype, device="cuda")
     if workspace is None:
         workspace = ie.paged_attention_workspace()
-        workspace.fill_(255)  # whatever it holds: NaN as floats
+        workspace[65536:].fill_(255)  # whatever it holds behind the counters: NaN as floats
     ie.paged_attention(s["q"], cache, s["table"], s["q_start"], s["kv_len"], out,
                        max_q=max(s["q_lens"] + [0]) if max_q is None else max_q, window=window, sinks=sinks,
                        scale=scale, workspace=workspace, **kw)
+    assert not bool(workspace[:65536].any())  # the counters are back at 0
     return out
 
 
