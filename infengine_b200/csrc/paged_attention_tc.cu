@@ -168,6 +168,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
   return r != 0;
 }
+// the n lowest bits (none for n <= 0, all from 32 on)
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+}
 // NaN if any operand is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -590,17 +594,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           for (int x = 0; x < kKB; ++x) v[x] = 0.f;
         }
         if (masked) {
+          // the columns the row sees, as bits
           const float hidden = c > 0.f ? -INFINITY : INFINITY;
-          const int hi = pos - kb;  // columns <= hi
-          if (!a.window) {
-#pragma unroll
-            for (int x = 0; x < kKB; ++x) v[x] = x <= hi ? v[x] : hidden;
-          } else {
-            const int64_t lo64 = (int64_t)pos - a.window - kb;
-            const int lo = (int)(lo64 < -1 ? -1 : lo64), sk = a.sinks - kb;  // columns > lo or < sk
-#pragma unroll
-            for (int x = 0; x < kKB; ++x) v[x] = x <= hi && (x > lo || x < sk) ? v[x] : hidden;
+          const int hi = pos - kb + 1;  // columns below hi
+          uint32_t see[2] = {low_bits(hi), low_bits(hi - 32)};
+          if (a.window) {
+            const int64_t lo64 = (int64_t)pos - a.window - kb + 1;
+            const int lo = (int)(lo64 < 0 ? 0 : lo64), sk = a.sinks - kb;  // but not those below lo, unless below sk
+            see[0] &= ~low_bits(lo) | low_bits(sk);
+            see[1] &= ~low_bits(lo - 32) | low_bits(sk - 32);
           }
+#pragma unroll
+          for (int x = 0; x < kKB; ++x) v[x] = see[x >> 5] >> (x & 31) & 1 ? v[x] : hidden;
         }
         // the row's largest scaled score
         float top;
