@@ -788,58 +788,55 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-// Joins the cut tiles' pieces in piece order, 32 rows (one warp's of the chunk
-// kernel) a CTA: a thread has one row, its warp every fourth 16-byte piece of
-// the row's outputs, as the chunk kernel stored them. The rows go out through
-// shared memory.
+// Joins the cut tiles' pieces in piece order: a CTA takes 32 rows (one warp's of
+// the chunk kernel) and 32 of their outputs, a thread one row and four outputs,
+// as the chunk kernel stored them. So small, because a few tiles in many pieces
+// are the common case and the reads' latency is what the join costs: a chunk of
+// 64 tokens over 8192 rows (8 tiles in 18 pieces) took 48 us with 128 threads
+// for 32 whole rows, and takes 31. The rows go out through shared memory.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_chunks_kernel(const __grid_constant__ Args a) {
-  constexpr int kMine = D / 16, kPitch = D * 2 + 8;
+__global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant__ Args a) {
+  constexpr int kParts = D / 32, kPitch = 32 * 2 + 8;
   __shared__ __align__(16) uint8_t rows_s[32 * kPitch];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nkv = a.l.n_kv_heads;
-  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * 8 * kParts;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const Split sp = a.splits[it >> 3];
-    const int part = (int)(it & 7), i = part >> 2, r0 = 32 * (part & 3);  // lane of the tile, first row there
-    if (r0 >= a.lane_rows || i * a.lane_rows + r0 >= sp.rows) continue;   // the same for the whole block
+    const int d0 = 32 * (int)(it % kParts), group = (int)(it / kParts % 8);
+    const Split sp = a.splits[it / (8 * kParts)];
+    const int i = group >> 2, r0 = 32 * (group & 3);                     // lane of the tile, first row there
+    if (r0 >= a.lane_rows || i * a.lane_rows + r0 >= sp.rows) continue;  // the same for the whole block
+    const int64_t step = a.l.n_kv_heads;
+    const float2* ml = a.part_ml + (int64_t)sp.slot0 * kRowsChunk + 32 * group + lane;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) +
+                       (((int64_t)sp.slot0 * 8 + group) * (D / 4) + d0 / 4 + warp) * 32 + lane;
     float top = -INFINITY;
-    for (int s = 0; s < sp.pieces; ++s)
-      top = fmaxf(top, a.part_ml[((int64_t)sp.slot0 + (int64_t)s * nkv) * kRowsChunk + 32 * part + lane].x);
-    float4 acc[kMine];
-#pragma unroll
-    for (int x = 0; x < kMine; ++x) acc[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < sp.pieces; ++s) top = fmaxf(top, ml[s * step * kRowsChunk].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-#pragma unroll 2
+#pragma unroll 8
     for (int s = 0; s < sp.pieces; ++s) {
-      const int64_t slot = (int64_t)sp.slot0 + (int64_t)s * nkv;
-      const float2 ml = a.part_ml[slot * kRowsChunk + 32 * part + lane];
-      const float f = top == -INFINITY ? 0.f : ex2(ml.x - top);
-      sum += f * ml.y;
-      const float4* po = reinterpret_cast<const float4*>(a.part_o) + (slot * 8 + part) * (D / 4) * 32 + lane;
-#pragma unroll
-      for (int x = 0; x < kMine; ++x) {
-        const float4 u = po[(warp + 4 * x) * 32];
-        acc[x].x += f * u.x;
-        acc[x].y += f * u.y;
-        acc[x].z += f * u.z;
-        acc[x].w += f * u.w;
-      }
+      const float2 x = ml[s * step * kRowsChunk];
+      const float4 u = po[s * step * 8 * (D / 4) * 32];
+      const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
+      sum += f * x.y;
+      acc.x += f * u.x;
+      acc.y += f * u.y;
+      acc.z += f * u.z;
+      acc.w += f * u.w;
     }
     const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-#pragma unroll
-    for (int x = 0; x < kMine; ++x)
-      *reinterpret_cast<uint2*>(rows_s + lane * kPitch + (warp + 4 * x) * 8) =
-          make_uint2(pack2<T>(acc[x].x * inv, acc[x].y * inv), pack2<T>(acc[x].z * inv, acc[x].w * inv));
+    *reinterpret_cast<uint2*>(rows_s + lane * kPitch + warp * 8) =
+        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
     __syncthreads();
-    constexpr int kLanes = D / 4, kRows = 128 / kLanes;  // 8 bytes a thread
-    for (int q = threadIdx.x / kLanes; q < 32; q += kRows) {
-      const int cc = threadIdx.x % kLanes, g = i * a.lane_rows + r0 + q;
-      if (r0 + q < a.lane_rows && g < sp.rows)
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(sp.token0 + g / a.group) * a.ld_out +
-                                  (int64_t)(sp.head0 + g % a.group) * D + 4 * cc) =
-            *reinterpret_cast<const uint2*>(rows_s + q * kPitch + cc * 8);
+    const int q = threadIdx.x >> 3, g = i * a.lane_rows + r0 + q;  // 8 threads a row, 8 bytes each
+    if (r0 + q < a.lane_rows && g < sp.rows) {
+      const int tok = g * a.group_magic >> 16;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(sp.token0 + tok) * a.ld_out +
+                                (int64_t)(sp.head0 + g - tok * a.group) * D + d0 + 4 * (threadIdx.x & 7)) =
+          *reinterpret_cast<const uint2*>(rows_s + q * kPitch + (threadIdx.x & 7) * 8);
     }
     __syncthreads();
   }
@@ -862,10 +859,10 @@ int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
   kernel<<<(unsigned)grid, kThreads, kControl + Cfg<D>::kTiles, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) {
-    const int64_t items = 8 * (most_tiles < a.target ? most_tiles : a.target);
+    const int64_t items = 8 * (D / 32) * (most_tiles < a.target ? most_tiles : a.target);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items < 148 * 8 ? items : 148 * 8));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
