@@ -282,7 +282,7 @@ typedef struct ie_paged_cache {
  * q_start[b + 1] - 1 (device array [B + 1], not decreasing; a sequence may own
  * none) and they sit at the last positions of its kv_len[b] cache rows (device
  * array [B], new rows included). T is the number of rows the buffers hold:
- * rows no sequence owns are not read and not written. page_table is a device
+ * rows no sequence owns may hold anything and are not written. page_table is a device
  * array [B][max_pages] (row stride ld_table); entries for rows nobody asks for
  * may hold anything. All three are read when the kernels run, so a captured
  * graph follows them. What lies outside the call's extents (a page outside

@@ -12,10 +12,10 @@
 // Layout: D/16 lanes serve a head (8 for D = 128, 4 for 64). A lane loads the
 // 16 bytes at dimension 8i and the 16 bytes at D/2 + 8i, so both members of
 // every rotated pair are in its registers and the norm needs 3 (or 2)
-// shuffles. A warp serves one token: it finds the token's sequence once (a
-// 32-ary search over q_start) and holds the position's cosines and sines in
-// registers for kHeads rounds of 32 / (D/16) heads, whose loads are all issued
-// before the first is used.
+// shuffles. A warp serves one token: it issues the loads of kHeads rounds of
+// 32 / (D/16) heads, finds the token's sequence (a 32-ary search over q_start)
+// and page meanwhile, and holds the position's cosines and sines in registers
+// for all its heads.
 #include "ie_common.cuh"
 #include "norm.cuh"
 #include "paged.cuh"
@@ -27,7 +27,7 @@ __device__ int g_paged_norm_status = 0;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMaxThreads = 256;
 
 struct NormArgs {
   PagedBatch b;
@@ -36,7 +36,7 @@ struct NormArgs {
   int64_t ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso;
   void *q_out, *kc, *vc;
   const float *cos, *sin;
-  int rope_rows, n_q, warps_per_token;
+  int rope_rows, n_q;
   float eps;
 };
 
@@ -58,33 +58,18 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
 template <typename T, int D, int kHeads>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
   constexpr int kLanes = D / 16;          // lanes of one head
   constexpr int kPerRound = 32 / kLanes;  // heads of one round
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t t = w / a.warps_per_token;
-  if (t >= a.b.T) return;
-  const int seq = paged_owner(a.b.q_start, a.b.B, (int)t);
-  if (seq < 0 || seq >= a.b.B) return;  // a row no sequence owns is left as it is
-  const int start = a.b.q_start[seq];
-  const int64_t pos64 = (int64_t)a.b.kv_len[seq] - ((int64_t)a.b.q_start[seq + 1] - start) + (t - start);
-  bool bad = pos64 < 0 || pos64 >= ((int64_t)a.b.max_pages << a.l.page_log2) || (a.cos && pos64 >= a.rope_rows);
-  const int pos = bad ? 0 : (int)pos64;
-  int page = 0;
-  if (!bad) page = a.b.page_table[(int64_t)seq * a.b.ld_table + (pos >> a.l.page_log2)];
-  bad = bad || page < 0 || page >= a.l.num_pages;
-  if (bad) {
-    if (lane == 0) atomicExch(&g_paged_norm_status, IE_ERR_INVALID_ARG);
-    return;
-  }
-  const int64_t row = (int64_t)page * a.l.page_stride + (int64_t)(pos & (a.l.page_size - 1)) * a.l.row_stride;
+  const int64_t t = blockIdx.x;
   const int d = 8 * (lane % kLanes);  // this lane's dimensions: d .. d + 7 and D/2 + d ..
   const int heads = a.n_q + 2 * a.l.n_kv_heads;
-  const int h0 = (int)(w % a.warps_per_token) * kHeads * kPerRound + lane / kLanes;
+  const int h0 = ((int)blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kHeads * kPerRound + lane / kLanes;
 
+  // the rows are on their way while the token's place is found
   uint4 lo[kHeads], hi[kHeads];
 #pragma unroll
   for (int r = 0; r < kHeads; ++r) {
@@ -101,6 +86,20 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormArgs a
       hi[r] = ld16(src + D / 2 + d);
     }
   }
+  const int seq = paged_owner(a.b.q_start, a.b.B, (int)t);
+  if (seq < 0 || seq >= a.b.B) return;  // a row no sequence owns is left as it is
+  const int start = a.b.q_start[seq];
+  const int64_t pos64 = (int64_t)a.b.kv_len[seq] - ((int64_t)a.b.q_start[seq + 1] - start) + (t - start);
+  bool bad = pos64 < 0 || pos64 >= ((int64_t)a.b.max_pages << a.l.page_log2) || (a.cos && pos64 >= a.rope_rows);
+  const int pos = bad ? 0 : (int)pos64;
+  int page = 0;
+  if (!bad) page = a.b.page_table[(int64_t)seq * a.b.ld_table + (pos >> a.l.page_log2)];
+  bad = bad || page < 0 || page >= a.l.num_pages;
+  if (bad) {
+    if (lane == 0) atomicExch(&g_paged_norm_status, IE_ERR_INVALID_ARG);
+    return;
+  }
+  const int64_t row = (int64_t)page * a.l.page_stride + (int64_t)(pos & (a.l.page_size - 1)) * a.l.row_stride;
   float c[8], s[8];
   if (a.cos) {
     const float4* cp = reinterpret_cast<const float4*>(a.cos + (int64_t)pos * (D / 2) + d);
@@ -165,13 +164,11 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormArgs a
 template <typename T, int D, int kHeads>
 int launch_heads(NormArgs& a, cudaStream_t st) {
   constexpr int kPerRound = 32 / (D / 16);
-  const int heads = a.n_q + 2 * a.l.n_kv_heads;
-  a.warps_per_token = ceil_div(heads, kPerRound * kHeads);
-  const int64_t blocks = ((int64_t)a.b.T * a.warps_per_token + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > INT_MAX) return IE_ERR_UNSUPPORTED;
+  const int warps = ceil_div(a.n_q + 2 * a.l.n_kv_heads, kPerRound * kHeads);
+  const int blocks = ceil_div(warps, kMaxThreads / 32);  // of a token, evenly filled
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)a.b.T, (unsigned)blocks);
+  cfg.blockDim = dim3(32u * ceil_div(warps, blocks));
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -184,10 +181,11 @@ int launch_heads(NormArgs& a, cudaStream_t st) {
 template <typename T, int D>
 int launch_norm(NormArgs& a, cudaStream_t st) {
   // One round of heads a warp while that leaves the GPU's warp slots unfilled
-  // (a decode step), else four.
+  // (a decode step), else three: with 11204 tokens of 32 + 8 + 8 heads one,
+  // two, three, four and six rounds took 78, 65, 55, 56 and 65 us.
   constexpr int kPerRound = 32 / (D / 16);
   const int64_t warps = (int64_t)a.b.T * ceil_div(a.n_q + 2 * a.l.n_kv_heads, kPerRound);
-  return warps <= 148 * 32 ? launch_heads<T, D, 1>(a, st) : launch_heads<T, D, 4>(a, st);
+  return warps <= 148 * 32 ? launch_heads<T, D, 1>(a, st) : launch_heads<T, D, 3>(a, st);
 }
 
 // rows of `heads` heads of D elements at the given strides
