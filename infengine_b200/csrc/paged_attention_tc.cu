@@ -772,6 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   __syncthreads();
   fence_after();
   if (*abort_flag && threadIdx.x == 0) {
+    atomicExch(a.n_split, 0);  // nothing to join
     // copies still in flight land before the CTA exits: the last queries, and
     // the last kDepth blocks of keys and values (an earlier one's stage was reused)
     auto landed = [&](uint32_t bar, uint32_t parity) {
@@ -805,6 +806,12 @@ __global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant_
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int d0 = 32 * (int)(it % kParts), group = (int)(it / kParts % 8);
     const Split sp = a.splits[it / (8 * kParts)];
+    // a chunk kernel that gave up may have left a description unwritten: nothing is taken on trust
+    if (sp.pieces < 1 || sp.pieces > a.slot_cap || sp.slot0 < 0 ||
+        sp.slot0 + (sp.pieces - 1) * (int64_t)a.l.n_kv_heads >= a.slot_cap || sp.rows < 1 || sp.rows > a.tile_rows ||
+        sp.token0 < 0 || sp.token0 + (int64_t)((sp.rows - 1) / a.group) >= a.b.T || sp.head0 < 0 ||
+        sp.head0 > (a.l.n_kv_heads - 1) * a.group)
+      continue;
     const int i = group >> 2, r0 = 32 * (group & 3);                     // lane of the tile, first row there
     if (r0 >= a.lane_rows || i * a.lane_rows + r0 >= sp.rows) continue;  // the same for the whole block
     const int64_t step = a.l.n_kv_heads;
