@@ -320,7 +320,7 @@ int ie_qk_norm_rope_paged(ie_dtype dt, int B, int T, int n_q_heads,
  * accumulation, the probabilities rounded to dt before the product with v;
  * zeros for a row that sees nothing. q as above (row stride ldq, head stride
  * q_head_stride); out [T][n_q_heads * head_dim], row stride ld_out, the input
- * of the O projection. max_q bounds the new tokens of one sequence; 1 is the
+ * of the O projection (out must overlap neither q nor the cache). max_q bounds the new tokens of one sequence; 1 is the
  * decode step. n_q_heads / n_kv_heads an integer up to 16.
  * A cache row that no row of its sequence sees (behind kv_len, outside every
  * window) may hold anything. Rows that are seen must be finite where another

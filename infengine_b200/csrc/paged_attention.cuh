@@ -179,6 +179,12 @@ __device__ __forceinline__ Piece piece_at(const Args& a, int b, int tiles, int S
   return p;
 }
 
+// Pieces of a tile of n blocks, about C = 1 / per each. (No integer division: a
+// wave of CTAs counts them for 32 sequences and 32 lengths before it starts.)
+__device__ __forceinline__ int pieces_of(int n, int C, float per) {
+  return n > C ? (int)((float)(n - 1) * per) + 1 : 1;
+}
+
 // Blocks of a piece where whole waves of a.wave CTAs count: lane k - 1 weighs
 // cutting the longest tile into k pieces of C = most / k blocks. With P pieces
 // of A blocks on average, W = ceil(P / wave) waves cost W (A + o) + C - A
@@ -190,18 +196,20 @@ __device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_he
   // (the last lanes: as many pieces as just fill one wave, and two)
   const int k = lane < 30 ? lane + 1 : max((lane - 29) * a.wave / max(all, 1), 1);
   const int C = max((longest - 1) / k + 1, 1);
-  long long pieces = 0, cut = 0, blocks = 0;
+  const float per = 1.0f / (float)C;
+  float pieces = 0.f, cut = 0.f, blocks = 0.f;
+#pragma unroll 4
   for (int b = 0; b < a.b.B; ++b) {
     const int t = __shfl_sync(0xffffffffu, tiles_heads, b), n = __shfl_sync(0xffffffffu, most, b);
-    const int S = n > C ? (n - 1) / C + 1 : 1;
-    pieces += (long long)t * S;
-    cut += S > 1 ? (long long)t * S : 0;
-    blocks += (long long)t * n;
+    const float p = (float)t * (float)pieces_of(n, C, per);
+    pieces += p;
+    cut += n > C ? p : 0.f;
+    blocks += (float)t * (float)n;
   }
-  const float avg = pieces ? (float)blocks / (float)pieces : 0.f;
-  const float waves = (float)((pieces + a.wave - 1) / a.wave);
-  float cost = waves * (avg + (cut ? a.cut : a.whole)) + (float)C - avg;
-  if (cut > a.slot_cap || pieces > a.max_pieces || (k > 1 && C < a.min_blocks)) cost = INFINITY;
+  const float avg = pieces > 0.f ? blocks / pieces : 0.f;
+  const float waves = ceilf(pieces / (float)a.wave);
+  float cost = waves * (avg + (cut > 0.f ? a.cut : a.whole)) + (float)C - avg;
+  if (cut > (float)a.slot_cap || pieces > (float)a.max_pieces || (k > 1 && C < a.min_blocks)) cost = INFINITY;
   float least = cost;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -288,7 +296,7 @@ struct Finder {
   }
   __device__ __forceinline__ void scan() {
     const int lane = threadIdx.x & 31, nkv = a.l.n_kv_heads;
-    S = most > C ? (most - 1) / C + 1 : 1;
+    S = pieces_of(most, C, 1.0f / (float)C);
     // a count past the range cannot be asked for: the host bounds the pieces
     mine = (int)min((long long)tiles * S * nkv, 1LL << 25);
     x = mine;
@@ -329,7 +337,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
         if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
       }
       const int C = piece_blocks_by_waves(a, tiles * nkv, most);
-      const int S = most > C ? (most - 1) / C + 1 : 1;
+      const int S = pieces_of(most, C, 1.0f / (float)C);
       // a count past the grid's range cannot be asked for: the host bounds the pieces
       const int mine = (int)min((long long)tiles * S * nkv, 1LL << 25);
       int x = mine, y = S > 1 ? mine : 0, z = S > 1 ? tiles * nkv : 0;
@@ -354,21 +362,19 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
     __syncthreads();
     return sc.found != 0;
   }
-  long long u = 0;
+  long long u[3] = {0, 0, 0}, sums[3];  // blocks, tiles
   for (int b = tid; b < a.b.B; b += THREADS) {
     const Seq s = sequence(a, b);
-    u += (long long)tile_count(a, s) * nkv * most_blocks<KB>(a, s);
+    const long long t = (long long)tile_count(a, s) * nkv;
+    u[0] += t * most_blocks<KB>(a, s);
+    u[1] += t;
     if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-  if ((tid & 31) == 0) sc.w[0][tid >> 5] = u;
   if (tid == 0) sc.found = 0;
-  __syncthreads();
-  u = 0;
-  for (int i = 0; i < THREADS / 32; ++i) u += sc.w[0][i];
-  __syncthreads();
-  const int C = piece_blocks(a, u);
+  block_scan3<THREADS>(u, sums, sc);
+  // lengths that contradict T could ask for more pieces than were launched:
+  // then no tile is cut, since a cut one needs all of its pieces
+  const int C = sums[1] + a.target > a.max_pieces ? INT_MAX / 2 : piece_blocks(a, sums[0]);
   long long run[3] = {0, 0, 0};  // pieces, slots, cut tiles so far
   for (int b0 = 0; b0 < a.b.B; b0 += THREADS) {
     const int b = b0 + tid;
@@ -379,7 +385,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
       s = sequence(a, b);
       const int most = most_blocks<KB>(a, s);
       tiles = tile_count(a, s);
-      S = most > C ? (most - 1) / C + 1 : 1;
+      S = pieces_of(most, C, 1.0f / (float)C);
       v[0] = (long long)tiles * S * nkv;
       v[1] = S > 1 ? v[0] : 0;
       v[2] = S > 1 ? (long long)tiles * nkv : 0;

@@ -591,6 +591,9 @@ extern "C" int ie_sample(ie_dtype dt, int M, int V, const void* logits, int64_t 
   if (V == 0 || !logits || !u || !idx_out) return IE_ERR_INVALID_ARG;
   if (M > (1 << 24)) return IE_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(logits) & 1u) return IE_ERR_ALIGNMENT;
+  for (const void* p : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p,
+                        (const void*)u, (const void*)idx_out, (const void*)logprob_out})
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return IE_ERR_ALIGNMENT;
   SampleArgs a = {logits, ld, V, temperature, top_p, min_p, u, top_k, idx_out, logprob_out};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dt == IE_DTYPE_F16 ? dispatch<__half>(a, M, st) : dispatch<__nv_bfloat16>(a, M, st);

@@ -61,7 +61,8 @@ def attention(lib, **kw):
     (dict(hs=64), -1), (dict(ldq=-8), -1), (dict(ldo=1016), -1),
     (dict(q=vp(0x1008)), -2), (dict(out=vp(0x1002)), -2), (dict(ldq=1028), -2), (dict(hs=132), -2),
     (dict(ldo=1028), -2), (dict(ws=None), -7), (dict(bytes=1000), -7), (dict(ws=vp(0x1004)), -2),
-    (dict(max_q=1 << 30, T=1 << 30), -3),
+    (dict(max_q=1 << 30, T=1 << 30), -3), (dict(table=vp(0x1002)), -2), (dict(start=vp(0x1001)), -2),
+    (dict(kv=vp(0x1002)), -2),
     (dict(B=0), 0), (dict(T=0), 0), (dict(max_q=0), 0),
 ])
 def test_attention_refusals(lib, change, status):
@@ -95,6 +96,7 @@ def test_norm_rope_refusals(lib, change, status):
 @pytest.mark.parametrize("change,status", [
     (dict(dt=3), -1), (dict(M=-1), -1), (dict(V=-1, ld=0), -1), (dict(V=0), -1), (dict(ld=99), -1),
     (dict(x=None), -1), (dict(u=None), -1), (dict(idx=None), -1), (dict(x=vp(0x1001)), -2),
+    (dict(u=vp(0x1002)), -2), (dict(idx=vp(0x1001)), -2),
     (dict(V=600000, ld=600000), -3), (dict(M=1 << 25), -3), (dict(M=0), 0),
 ])
 def test_sample_refusals(lib, change, status):
