@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
     const int64_t stride = (int64_t)a.l.n_kv_heads * kMT, first = (int64_t)pc.slot * kMT - pc.piece * stride;
     const float2* ml = a.part_ml + first + min(lane, kMT - 1);
     float most = -INFINITY, total = 0.f;
-#pragma unroll 8
+#pragma unroll 4
     for (int s = warp; s < pc.pieces; s += kWarps) most = fmaxf(most, __ldcg(ml + s * stride).x);
 #pragma unroll 1
     for (int q0 = 0; q0 < nrows; q0 += 4) {
@@ -674,7 +674,7 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   a.target = kTargetFew;
   a.wave = 2 * 148;
   a.whole = 5;
-  a.cut = 9;
+  a.cut = 20;
   a.min_blocks = 4;
   a.slot_cap = 2 * kTargetFew;
   const int64_t grid = tiles(kRowsFew) + (B <= 32 ? a.wave : a.target);
