@@ -71,7 +71,7 @@ def attention(s, window=0, sinks=0, scale=None):
       u |o|         the output's rounding
       2 A e         e the relative error of a p in fp32: the score's dot product
                     (D + 2 terms of 2^-23 of sum |q_i k_i|), its scaling and the
-                    exponential (2^-20), and the running sums of n terms (n / 16
+                    exponential (2^-18), and the running sums of n terms (n / 16
                     steps and 64 joins of 2^-23, on both sums)."""
     dim, group = s["dim"], s["heads"] // s["kv_heads"]
     scale = dim ** -0.5 if scale is None else scale
@@ -101,7 +101,7 @@ def attention(s, window=0, sinks=0, scale=None):
         o = (e @ v) / total
         A = (e @ v.abs()) / total
         dots = (q.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
-        err = (dim + 2) * 2.0 ** -23 * dots + 2.0 ** -20 + (kv / 16 + 64) * 2.0 ** -23
+        err = (dim + 2) * 2.0 ** -23 * dots + 2.0 ** -18 + (kv / 16 + 64) * 2.0 ** -23
         out[t] = o.transpose(0, 1)
         bound[t] = (u * (A + 2 * o.abs()) + 2 * A * err).transpose(0, 1)
     tiny = torch.finfo(s["q"].dtype).smallest_normal * torch.finfo(s["q"].dtype).eps
