@@ -486,12 +486,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             }
           continue;
         }
-        auto qk = [&](int j) {  // scores of block j, into the buffer of block g + j - 2
+        auto k_there = [&](int j) { return over(full_bar((gc + j) % kDepth), phase(gc + j)); };
+        auto qk = [&](int j) {  // scores of block j, into the buffer of block g + j - 2; its keys are there
           const int s = (gc + j) % kDepth, b = (g + j) & 1;
-          if (g + j >= 2 && !over(pv_done(i, b), (uint32_t)(((g + j - 2) >> 1) & 1))) return false;
-          if (!over(full_bar(s), phase(gc + j))) return false;
-          fence_after();
           const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
+          if (g + j >= 2 && !over(pv_done(i, b), (uint32_t)(((g + j - 2) >> 1) & 1))) return false;
+          fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
@@ -505,10 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         };
         ok = over(q_full, (uint32_t)(queries & 1));
         ++queries;
-        for (int j = 0; ok && j < min(n, 2); ++j) ok = qk(j);
+        for (int j = 0; ok && j < min(n, 2); ++j) ok = k_there(j) && qk(j);
         // the epilogue has read the last tile's outputs
         if (ok && tiles > 0) ok = over(o_empty(i), (uint32_t)((tiles - 1) & 1));
         for (int j = 0; ok && j < n; ++j) {
+          // what can be waited for before P is: this block's values, the keys of the next but one
           const int s = kDepth + (gc + j) % kDepth, kb = it.keys.block(it.j0 + j) * kKB, b = (g + j) & 1;
           if (!(ok = over(full_bar(s), phase(gc + j)))) break;
           if (kb + kKB > it.keys.hi || (kb < it.keys.lo && kb + kKB > it.keys.sink_end)) {
@@ -525,9 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
+          if (j + 2 < n && !(ok = k_there(j + 2))) break;
+          const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
           if (!(ok = over(p_full(i, b), (uint32_t)(((g + j) >> 1) & 1)))) break;
           fence_after();
-          const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kKB / 16; ++k)
