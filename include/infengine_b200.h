@@ -282,13 +282,14 @@ typedef struct ie_paged_cache {
  * q_start[b + 1] - 1 (device array [B + 1], not decreasing; a sequence may own
  * none) and they sit at the last positions of its kv_len[b] cache rows (device
  * array [B], new rows included). T is the number of rows the buffers hold:
- * rows no sequence owns may hold anything and are not written. page_table is a device
- * array [B][max_pages] (row stride ld_table); entries for rows nobody asks for
- * may hold anything. All three are read when the kernels run, so a captured
- * graph follows them. What lies outside the call's extents (a page outside
- * the pool, more rows than max_pages pages hold, more than max_q new tokens of
- * one sequence, a row outside T) is not accessed: it sets IE_ERR_INVALID_ARG
- * in ie_device_status, and the rows concerned are undefined. */
+ * rows no sequence owns may hold anything and are not written. page_table is a
+ * device array [B][max_pages] (row stride ld_table; max_pages * page_size below
+ * 2^31 - 1023); entries for rows nobody asks for may hold anything. All three
+ * are read when the kernels run, so a captured graph follows them. What lies
+ * outside the call's extents (a page outside the pool, more rows than max_pages
+ * pages hold, more than max_q new tokens of one sequence, a row outside T) is
+ * not accessed: it sets IE_ERR_INVALID_ARG in ie_device_status, and the rows
+ * concerned are undefined. */
 
 /* Per-head RMSNorm and rotation of the new tokens' queries and keys, with
  * keys and values written to their pages, in one pass: for each head row x of
@@ -320,17 +321,18 @@ int ie_qk_norm_rope_paged(ie_dtype dt, int B, int T, int n_q_heads,
  * accumulation, the probabilities rounded to dt before the product with v;
  * zeros for a row that sees nothing. q as above (row stride ldq, head stride
  * q_head_stride); out [T][n_q_heads * head_dim], row stride ld_out, the input
- * of the O projection (out must overlap neither q nor the cache). max_q bounds the new tokens of one sequence; 1 is the
- * decode step. n_q_heads / n_kv_heads an integer up to 16.
+ * of the O projection (out must overlap neither q nor the cache). max_q bounds
+ * the new tokens of one sequence; 1 is the decode step. n_q_heads / n_kv_heads
+ * an integer up to 16.
  * A cache row that no row of its sequence sees (behind kv_len, outside every
  * window) may hold anything. Rows that are seen must be finite where another
  * row of the same sequence does not see them: 0 * infinity is not 0.
  * workspace: ie_paged_attention_workspace_size() bytes, 16-byte aligned, its
  * first 64 KB zeroed once when allocated; every call leaves them zeroed again.
  * Calls that share one must not overlap on the GPU (one stream, or ordered
- * streams, and not two captured graphs that may run at once). The same call gives the same bits
- * every time; a row's last bits may depend on the other sequences of the
- * batch, which decide how the work is divided. */
+ * streams, and not two captured graphs that may run at once). The same call
+ * gives the same bits every time; a row's last bits may depend on the other
+ * sequences of the batch, which decide how the work is divided. */
 size_t ie_paged_attention_workspace_size(void);
 int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_heads,
                        const void* q, int64_t ldq, int64_t q_head_stride,
@@ -406,8 +408,9 @@ int ie_argmax(ie_dtype dt, int M, int V, const void* logits, int64_t ld,
  *          top_p times the mass of the top_k;
  *   min_p  (NULL or <= 0: off) keeps those with w >= min_p;
  * the first token is always kept. idx_out gets the first token whose running
- * mass exceeds u times the kept mass (u in [0, 1); a larger u gives the last
- * kept token), logprob_out (nullable) the log of its share of the kept mass.
+ * mass exceeds u times the kept mass (u in [0, 1); a smaller u counts as 0, a
+ * larger one and NaN give the last kept token), logprob_out (nullable) the log
+ * of its share of the kept mass.
  * temperature (NULL: 1) not above 0, NaN included: the first token, logprob 0.
  * Masses are 64-bit sums over the distinct values, so the ids do not depend
  * on an order of summation. -infinity and NaN logits are never sampled;

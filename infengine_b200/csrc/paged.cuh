@@ -48,8 +48,8 @@ inline int check_paged(const ie_paged_cache* c, int B, int T, const int* page_ta
   if (!page_table || !q_start || !kv_len || max_pages <= 0 || ld_table < max_pages) return IE_ERR_INVALID_ARG;
   for (const void* p : {(const void*)page_table, (const void*)q_start, (const void*)kv_len})
     if (reinterpret_cast<uintptr_t>(p) & 3u) return IE_ERR_ALIGNMENT;
-  // positions are 32-bit
-  if ((int64_t)max_pages * ps > INT_MAX) return IE_ERR_INVALID_ARG;
+  // positions are 32-bit, rounded up to whole blocks of keys and tiles of tokens included
+  if ((int64_t)max_pages * ps > INT_MAX - 1023) return IE_ERR_INVALID_ARG;
   return IE_OK;
 }
 

@@ -616,7 +616,8 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   if (!(scale > -INFINITY && scale < INFINITY)) return IE_ERR_INVALID_ARG;
   if (sinks && !window) return IE_ERR_INVALID_ARG;
   if (B == 0 || T == 0 || max_q == 0) return IE_OK;
-  if (!q || !out || q_head_stride < D || (T > 1 ? ldq < D : ldq < 0) || ld_out < (int64_t)n_q_heads * D) return IE_ERR_INVALID_ARG;
+  if (!q || !out || q_head_stride < D || (T > 1 ? ldq < D : ldq < 0) || ld_out < (int64_t)n_q_heads * D)
+    return IE_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(out) || ldq % 8 || q_head_stride % 8 || ld_out % 8) return IE_ERR_ALIGNMENT;
   if ((int64_t)max_q * group > INT_MAX - kRowsChunk || (int64_t)T * group > INT_MAX - kRowsChunk)
     return IE_ERR_UNSUPPORTED;

@@ -8,8 +8,8 @@
 // blocks of KB keys (aligned; sink rows first). A tile with many blocks is cut
 // into S pieces of at most C blocks each, where C is chosen from the whole
 // batch so that the pieces fill the GPU; the pieces' unnormalised outputs,
-// maxima and sums meet in the workspace and a second kernel joins them in
-// piece order. All of it is computed on the device from the lengths, so a
+// maxima and sums meet in the workspace and are joined in piece order (by the
+// tile's last CTA or by a second kernel). All of it is computed on the device from the lengths, so a
 // captured graph follows them.
 #pragma once
 #include <cuda.h>
@@ -230,7 +230,6 @@ struct Finder {
   int rx, ry, rz;               // of the sequences before b0
 
   __device__ __forceinline__ explicit Finder(const Args& args, int* status) : a(args) {
-    const int lane = threadIdx.x & 31;
     const bool tell = blockIdx.x == 0;
     if (a.b.B <= 32) {
       read(0, tell, status);
@@ -263,11 +262,10 @@ struct Finder {
       read(0, false, status);
       scan();
     }
-    (void)lane;
   }
   // Piece `index` (at least the last one asked for); true in the lane that has it.
   __device__ __forceinline__ bool find(int index, Piece& p, int* status) {
-    while (index >= rx + __shfl_sync(0xffffffffu, x, 31)) {  // index < total
+    while (index >= rx + __shfl_sync(0xffffffffu, x, 31) && b0 + 32 < a.b.B) {
       skip();
       read(b0 + 32, false, status);
       scan();
@@ -400,7 +398,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
     }
 #pragma unroll
     for (int j = 0; j < 3; ++j) run[j] += total[j];
-    if (index != 0 && run[0] > index) break;
+    if (run[0] > index) break;
   }
   __syncthreads();
   return sc.found != 0;

@@ -426,10 +426,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         for (int t = 0;; ++t) {
           if (!over(item_empty(t), (uint32_t)(((t >> 1) & 1) ^ 1))) break;
           const int index = t * G + ((t & 1) ? G - 1 - c : c);
-          const bool more = index < finder.total;
+          bool more = index < finder.total;
           if (more) {
             Piece p;
-            if (finder.find(index, p, &g_paged_tc_status)) {
+            const bool mine = finder.find(index, p, &g_paged_tc_status);
+            more = __any_sync(0xffffffffu, mine);
+            if (mine) {
               const Seq& sq = finder.s;
               const int row0 = p.tile * a.tile_rows, per = a.tile_rows / a.group, tok0 = p.tile * per;
               Item x;
@@ -447,9 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               x.pieces = p.pieces;
               ctl.items[t & 1] = x;
             }
-          } else if (lane == 0) {
-            ctl.items[t & 1].n = -1;
           }
+          if (!more && lane == 0) ctl.items[t & 1].n = -1;
           __syncwarp();
           it = ctl.items[t & 1];
           __syncwarp();

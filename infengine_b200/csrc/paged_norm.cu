@@ -190,7 +190,7 @@ int launch_norm(NormArgs& a, cudaStream_t st) {
 
 // rows of `heads` heads of D elements at the given strides
 int check_rows(const void* p, int64_t ld, int64_t hs, int D) {
-  if (!p || ld < 0 || hs < D) return IE_ERR_INVALID_ARG;
+  if (!p || ld < 0 || hs < D || ld > (INT64_C(1) << 40) || hs > (INT64_C(1) << 40)) return IE_ERR_INVALID_ARG;
   if (!aligned16(p) || ld % 8 || hs % 8) return IE_ERR_ALIGNMENT;
   return IE_OK;
 }
@@ -229,7 +229,10 @@ extern "C" int ie_qk_norm_rope_paged(ie_dtype dt, int B, int T, int n_q_heads, c
   if ((s = check_rows(q, ldq, q_head_stride, D)) || (s = check_rows(k, ldk, k_head_stride, D)) ||
       (s = check_rows(v, ldv, v_head_stride, D)) || (s = check_rows(q_out, ldo, o_head_stride, D)))
     return s;
-  if (T > 1 && ldo < D) return IE_ERR_INVALID_ARG;  // output rows must not coincide
+  // output rows must not overlap: tokens outside heads or heads outside tokens
+  if (T > 1 && !(ldo >= (n_q_heads - 1) * o_head_stride + D ||
+                 (ldo >= D && (n_q_heads == 1 || o_head_stride >= (T - 1) * ldo + D))))
+    return IE_ERR_INVALID_ARG;
   if ((q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)) ||
       (rope_cos && (!aligned16(rope_cos) || !aligned16(rope_sin))))
     return IE_ERR_ALIGNMENT;

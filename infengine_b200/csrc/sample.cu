@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
             }
           }
         }
-        const double border = greedy ? 0.0 : (double)a.u[row] * Z;
+        const float u = a.u[row];
+        const double border = greedy || u < 0.f ? 0.0 : (double)u * Z;
         Lane v = values(group_of([&](int g) { return mass_at(g) > border; }));
         const unsigned any = __ballot_sync(0xffffffffu, v.n != 0);
         const unsigned over = __ballot_sync(0xffffffffu, v.n && v.before_m + v.n * v.w > border);

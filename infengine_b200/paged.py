@@ -139,6 +139,8 @@ def paged_attention(q, cache, page_table, q_start, kv_len, out, max_q, window=0,
             workspace.record_stream(other)
     if not q.get_device() == out.get_device() == workspace.get_device() == dev:
         raise ValueError(_ONE_DEVICE)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace is not contiguous")
     s = (_calls or _bind())[0](
         cache.code, B, T, max_q, heads, q.data_ptr(), ldq, hs, cache._ref, page_table.data_ptr(), ld_table, wide,
         q_start.data_ptr(), kv_len.data_ptr(), window, sinks, dim ** -0.5 if scale is None else scale, out.data_ptr(),

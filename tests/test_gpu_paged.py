@@ -336,3 +336,94 @@ def test_norm_rope_bad_extents_set_the_status(ie, cuda):
     assert bool((out[0] == 77.0).all()) and bool((out[2] == 77.0).all()) and bool((out[1] == x[1, :2]).all())
     at = int(s["table"][1, 39 // 16])
     assert bool((s["v"][at, 0, 39 % 16] == x[1, 3]).all())
+
+
+# -------------------------------------------------- batches of other shapes
+def many(B, longest, most_new, seed):
+    """B sequences of 0 .. most_new new tokens, one of them far longer than the others."""
+    g = __import__("random").Random(seed)
+    q_lens = [g.choice([0, 1, 1, most_new, g.randint(1, most_new)]) for _ in range(B)]
+    kv_lens = [n + g.randint(0, 150) for n in q_lens]
+    q_lens[B // 2], kv_lens[B // 2] = most_new, longest
+    return q_lens, kv_lens
+
+
+@pytest.mark.parametrize("B", [32, 33, 64, 150, 300])
+@pytest.mark.parametrize("most_new,longest", [(1, 6000), (6, 900), (40, 5000)])
+def test_attention_many_sequences(ie, cuda, B, most_new, longest):
+    q_lens, kv_lens = many(B, longest, most_new, B + most_new)
+    check_attention(ie, cuda, ref.make_batch(q_lens, kv_lens, heads=4, kv_heads=1, dim=64, page=32, seed=B))
+    if most_new == 6:
+        check_attention(ie, cuda, ref.make_batch(q_lens, kv_lens, heads=4, kv_heads=1, dim=64, page=32, seed=B),
+                        window=40, sinks=3)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [60, 300]), ([50, 3], [60, 400])])
+def test_attention_rows_outside_the_batch(ie, cuda, q_lens, kv_lens):
+    """Rows before the first and behind the last sequence hold NaN: they are
+    neither written nor felt."""
+    s = ref.make_batch(q_lens, kv_lens, seed=21)
+    want = check_attention(ie, cuda, s)
+    T, heads, dim = s["q"].shape
+    q = cuda.full((T + 9, heads, dim), float("nan"), dtype=s["q"].dtype, device="cuda")
+    q[4:4 + T] = s["q"]
+    out = run_attention(ie, cuda, dict(s, q=q, q_start=s["q_start"] + 4))
+    assert ie.device_status() == 0
+    assert bool((out[4:4 + T] == want).all())
+    assert bool((out[:4] == 77.0).all()) and bool((out[4 + T:] == 77.0).all())
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_attention_shared_pages(ie, cuda, n):
+    """Sequences that begin with the same pages, and one listed twice."""
+    s = ref.make_batch([n, n, n], [200, 230, 200], seed=22)
+    s["table"][1, :8] = s["table"][0, :8]
+    s["table"][2] = s["table"][0]
+    out = check_attention(ie, cuda, s)
+    s["q"][2 * n:] = s["q"][:n]
+    out = check_attention(ie, cuda, s)
+    assert bool((out[2 * n:] == out[:n]).all())
+
+
+def test_attention_two_calls_at_once(ie, cuda):
+    """Two streams, a workspace each: both as they are alone."""
+    batches = [ref.make_batch([1], [30000], dim=64, page=64, seed=23), ref.make_batch([70], [9000], page=64, seed=24),
+               ref.make_batch([2, 1], [7000, 50], page=64, seed=25)]
+    want = [check_attention(ie, cuda, s) for s in batches]
+    streams = [cuda.cuda.Stream() for _ in batches]
+    ws = [ie.paged_attention_workspace() for _ in batches]
+    caches = [ie.PagedCache(s["k"], s["v"]) for s in batches]
+    outs = [[cuda.zeros_like(w) for _ in range(6)] for w in want]
+    cuda.cuda.synchronize()
+    for x in range(6):
+        for s, c, o, w, st in zip(batches, caches, outs, ws, streams):
+            ie.paged_attention(s["q"], c, s["table"], s["q_start"], s["kv_len"], o[x], max_q=max(s["q_lens"]),
+                               workspace=w, stream=st)
+    cuda.cuda.synchronize()
+    assert ie.device_status() == 0
+    for o, w in zip(outs, want):
+        assert all(bool((y == w).all()) for y in o)
+
+
+@pytest.mark.parametrize("B", [3, 40])
+@pytest.mark.parametrize("n", [4, 40])
+def test_attention_starts_that_decrease(ie, cuda, B, n):
+    """Starts out of order are reported; counters and later calls stay sound."""
+    s = ref.make_batch([n] * B, [900] * B, heads=4, kv_heads=1, dim=64, page=64, seed=26)
+    want = check_attention(ie, cuda, s)
+    start = s["q_start"].clone()
+    start[1::2] = 0
+    run_attention(ie, cuda, dict(s, q_start=start))
+    assert ie.device_status() == -1
+    run_attention(ie, cuda, dict(s, q_start=start.flip(0) - n))
+    assert ie.device_status() == -1
+    assert bool((check_attention(ie, cuda, s) == want).all())
+
+
+def test_attention_workspace_refusals(ie, cuda):
+    s = ref.make_batch([1], [9], seed=27)
+    n = ie.paged_attention_workspace_bytes()
+    with pytest.raises(ie.IEError):
+        run_attention(ie, cuda, s, workspace=cuda.zeros(n - 1, dtype=cuda.uint8, device="cuda"))
+    with pytest.raises(ValueError, match="contiguous"):
+        run_attention(ie, cuda, s, workspace=cuda.zeros(16, dtype=cuda.uint8, device="cuda")[:1].expand(n))

@@ -138,6 +138,20 @@ def test_u_at_the_ends(ie, cuda):
     assert idx.tolist() == [int(order[0, 0])] + [int(order[r, 9]) for r in (1, 2, 3)]
 
 
+def test_parameters_outside_their_ranges(ie, cuda):
+    """A negative u counts as 0; top_p of 0 or less, min_p above 1 and NaN of
+    either keep the first token alone."""
+    x, _, _ = inputs(cuda, 6, 500, "bf16", 2)
+    first = cuda.sort(x.float(), dim=-1, descending=True, stable=True).indices[:, 0].tolist()
+    f = lambda *v: cuda.tensor(v, device="cuda")  # noqa: E731
+    idx, lp = run(ie, cuda, x, f(-0.5, -0.0, -math.inf, -1e-30, 0.0, -2.0))
+    assert idx.tolist() == first
+    u = cuda.full((6,), 0.9, device="cuda")
+    idx, lp = run(ie, cuda, x, u, top_p=f(0.0, -1.0, math.nan, 1e-30, 1.0, 1.0),
+                  min_p=f(0.0, 0.0, 0.0, 0.0, 1.5, math.nan))
+    assert idx.tolist() == first and lp.tolist() == [0.0] * 6
+
+
 def test_a_row_does_not_depend_on_the_batch(ie, cuda):
     """1, 2, 4 and 8 CTAs a row give the same ids and log probabilities."""
     x, u, g = inputs(cuda, 160, 20011, "bf16", 3)

@@ -56,6 +56,7 @@ def attention(lib, **kw):
     (dict(cache=None), -1), (dict(heads=9), -3), (dict(heads=34), -3), (dict(q=None), -1), (dict(out=None), -1),
     (dict(table=None), -1), (dict(start=None), -1), (dict(kv=None), -1), (dict(pages=0), -1), (dict(ldt=7), -1),
     (dict(pages=1 << 28, ldt=1 << 28), -1),      # positions past 32 bits
+    (dict(pages=(1 << 27) - 8, ldt=1 << 28), -1),  # and those whose last block's end is
     (dict(window=-1), -1), (dict(sinks=-1), -1), (dict(sinks=4), -1),  # sinks without a window
     (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1),
     (dict(hs=64), -1), (dict(ldq=-8), -1), (dict(ldo=1016), -1),
@@ -87,7 +88,9 @@ def norm(lib, **kw):
     (dict(start=None), -1), (dict(kv=None), -1), (dict(cos=None), -1), (dict(sin=None), -1), (dict(rows=0), -1),
     (dict(eps=-1.0), -1), (dict(eps=float("nan")), -1), (dict(hq=64), -1), (dict(ho=64), -1), (dict(ldo=8), -1),
     (dict(q=vp(0x1008)), -2), (dict(kw=vp(0x1008)), -2), (dict(cos=vp(0x1004)), -2), (dict(ldk=1540), -2),
-    (dict(hv=130), -2), (dict(heads=70000, ldo=70000 * 128), -3), (dict(B=0), 0), (dict(T=0), 0),
+    (dict(hv=130), -2), (dict(ldq=1 << 41), -1), (dict(ho=1 << 41), -1),
+    (dict(ldo=7 * 128), -1), (dict(ldo=128, ho=3 * 128), -1), (dict(ldo=136, ho=3 * 136), -1),  # output rows overlap
+    (dict(heads=70000, ldo=70000 * 128), -3), (dict(B=0), 0), (dict(T=0), 0),
 ])
 def test_norm_rope_refusals(lib, change, status):
     assert norm(lib, **change) == status
