@@ -563,14 +563,14 @@ int launch_few(Args& a, int64_t grid, cudaStream_t st) {
                 args);
 }
 
-// workspace: pieces done of each tile (few rows; zeroed by the caller once) |
+// workspace: pieces done of each tile (few rows) and handed out (chunks), zeroed by the caller once |
 // number of cut tiles | their descriptions (chunks) | (maximum, sum) | outputs
 constexpr int kCapSplits = kTargetFew > kTargetChunk ? kTargetFew : kTargetChunk;
 constexpr int64_t kSlotRowsFew = (int64_t)2 * kTargetFew * kRowsFew;
 constexpr int64_t kSlotRowsChunk = (int64_t)2 * kTargetChunk * kRowsChunk;
 constexpr int64_t kSlotRows = kSlotRowsFew > kSlotRowsChunk ? kSlotRowsFew : kSlotRowsChunk;
-constexpr size_t kOffCount = 65536;
-static_assert(kCapSplits * sizeof(int) <= kOffCount, "counters");
+constexpr size_t kOffCount = 65536, kOffQueue = kOffCount - 64;
+static_assert(kCapSplits * sizeof(int) <= kOffQueue, "counters");
 constexpr size_t kOffSplits = kOffCount + 64;
 constexpr size_t kOffMl = kOffSplits + kCapSplits * sizeof(Split);
 constexpr size_t kOffO = kOffMl + kSlotRows * sizeof(float2);
@@ -657,8 +657,10 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
   if (!few) {
     a.n_split = reinterpret_cast<int*>(ws + kOffCount);
     a.wave = 148;
-    a.whole = 2;
+    a.whole = 4;
     a.cut = 6;
+    a.join = 6;
+    a.queue = reinterpret_cast<int*>(ws + kOffQueue);
     a.max_pieces = INT_MAX;
     a.group_magic = 65536 / group + 1;
     a.lane_rows = kRowsChunk / 2 / group * group;

@@ -40,9 +40,11 @@ struct Args {
   int wave;       // CTAs that run at once
   int max_pieces; // few rows: CTAs of the launch (a CTA without a piece costs its start)
   int whole, cut; // start and end of a piece, in blocks
+  int join;       // chunks: the joining kernel's time, in blocks
   int min_blocks; // smallest piece
   int slot_cap, split_cap;
   int* arrived;   // few rows: pieces done of each cut tile, 0 between calls
+  int* queue;     // chunks: pieces handed out behind the first of each CTA, 0 between calls
   int* n_split;   // chunks: number of cut tiles, and what the joining kernel needs of each
   Split* splits;
   float2* part_ml;  // [slot][row] (maximum in log2 units, sum)
@@ -217,6 +219,38 @@ __device__ __forceinline__ int piece_blocks_by_waves(const Args& a, int tiles_he
   return __shfl_sync(0xffffffffu, C, max(who, 0));
 }
 
+// The same for pieces that a.wave CTAs take from a queue, sequences in
+// descending order of their most blocks. A sequence's last piece ends at about
+// the work up to there divided by the CTAs, and half a piece (the first one's
+// pieces: in whole waves); the joining kernel adds a.join blocks and 1 / 25 a
+// partial result.
+__device__ __forceinline__ int piece_blocks_by_ends(const Args& a, int tiles_heads, int most) {
+  const int lane = threadIdx.x & 31;
+  const int longest = __shfl_sync(0xffffffffu, most, 0), all = __reduce_add_sync(0xffffffffu, tiles_heads);
+  const int k = lane < 30 ? lane + 1 : max((lane - 29) * a.wave / max(all, 1), 1);
+  const int C = max((longest - 1) / k + 1, 1);
+  const float per = 1.0f / (float)C, each = 1.0f / (float)a.wave;
+  float slots = 0.f, work = 0.f, cost = 0.f;
+#pragma unroll 4
+  for (int b = 0; b < a.b.B; ++b) {
+    const int t = __shfl_sync(0xffffffffu, tiles_heads, b), n = __shfl_sync(0xffffffffu, most, b);
+    const int S = pieces_of(n, C, per);
+    const float pieces = (float)t * (float)S;
+    const float size = __fdividef((float)n, (float)S) + (float)(n > C ? a.cut : a.whole);
+    slots += n > C ? pieces : 0.f;
+    work += pieces * size;
+    const float end = b == 0 ? ceilf(pieces * each) * size : work * each + 0.5f * size;
+    cost = t ? fmaxf(cost, end) : cost;
+  }
+  if (slots > 0.f) cost += (float)a.join + 0.04f * slots;
+  if (slots > (float)a.slot_cap || (k > 1 && C < a.min_blocks)) cost = INFINITY;
+  float least = cost;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  const int who = __ffs(__ballot_sync(0xffffffffu, cost == least)) - 1;
+  return __shfl_sync(0xffffffffu, C, max(who, 0));
+}
+
 // Finds pieces for one warp, in increasing order of their index: sequences are
 // taken 32 at a time, one a lane. The first 32 are read once; the pieces'
 // length comes from the whole batch (by waves for up to 32 sequences).
@@ -228,12 +262,14 @@ struct Finder {
   Seq s;
   int tiles, S, mine, x, y, z;  // this lane's; x, y, z inclusive sums of pieces, slots, cut tiles
   int rx, ry, rz;               // of the sequences before b0
+  int seq;                      // this lane's sequence
 
   __device__ __forceinline__ explicit Finder(const Args& args, int* status) : a(args) {
     const bool tell = blockIdx.x == 0;
     if (a.b.B <= 32) {
       read(0, tell, status);
-      C = piece_blocks_by_waves(a, tiles * a.l.n_kv_heads, most);
+      if (a.b.B > 1) longest_first();
+      C = piece_blocks_by_ends(a, tiles * a.l.n_kv_heads, most);
     } else {
       long long u = 0;
       for (int b = 0; b < a.b.B; b += 32) {
@@ -273,7 +309,7 @@ struct Finder {
     const int at = index - rx - (x - mine);
     if (at < 0 || at >= mine) return false;
     const int nkv = a.l.n_kv_heads;
-    p = piece_at(a, b0 + (threadIdx.x & 31), tiles, S, at, ry + y - (S > 1 ? mine : 0),
+    p = piece_at(a, seq, tiles, S, at, ry + y - (S > 1 ? mine : 0),
                  rz + z - (S > 1 ? tiles * nkv : 0));
     return true;
   }
@@ -285,12 +321,34 @@ struct Finder {
     s = {};
     tiles = most = 0;
     const int b = first + (threadIdx.x & 31);
+    seq = b;
     if (b < a.b.B) {
       s = sequence(a, b);
       tiles = tile_count(a, s);
       most = most_blocks<KB>(a, s);
       if (s.bad && tell) atomicExch(status, IE_ERR_INVALID_ARG);
     }
+  }
+  // Sequences in descending order of their most blocks, so that the last pieces
+  // handed out are short.
+  __device__ __forceinline__ void longest_first() {
+    const int lane = threadIdx.x & 31;
+    int rank = 0, from = 0;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+      const int n = __shfl_sync(0xffffffffu, most, i);
+      rank += n > most || (n == most && i < lane);
+    }
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i)
+      if (__shfl_sync(0xffffffffu, rank, i) == lane) from = i;
+    s.start = __shfl_sync(0xffffffffu, s.start, from);
+    s.tokens = __shfl_sync(0xffffffffu, s.tokens, from);
+    s.kv = __shfl_sync(0xffffffffu, s.kv, from);
+    s.pos0 = __shfl_sync(0xffffffffu, s.pos0, from);
+    tiles = __shfl_sync(0xffffffffu, tiles, from);
+    most = __shfl_sync(0xffffffffu, most, from);
+    seq = from;
   }
   __device__ __forceinline__ void scan() {
     const int lane = threadIdx.x & 31, nkv = a.l.n_kv_heads;

@@ -30,10 +30,11 @@
 // Operands are 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K
 // K-major, V MN-major as it arrives.
 //
-// One CTA an SM takes pieces in a back-and-forth order (c, 2G - 1 - c, 2G + c,
-// ..; the longest come first) until none is left, and every role runs ahead
-// of the next as far as its buffers allow: a CTA for each piece spent 10 us of
-// a 30 us piece on finding it, the first copies and the epilogue.
+// One CTA an SM takes pieces from a queue (the longest come first) until none
+// is left, and every role runs ahead of the next as far as its buffers allow: a
+// CTA for each piece spent 10 us of a 30 us piece on finding it, the first
+// copies and the epilogue; a fixed share of the pieces for each CTA left a
+// ragged batch of 10 to 800 tokens over up to 5000 rows at 297 us for 194.
 //
 // Warp roles: 0 finds the pieces and copies queries and keys, 2 values (TMA
 // boxes of up to 64 rows of one page; the lanes hold the next table entries),
@@ -351,10 +352,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const int box_log2 = min(a.l.page_log2, 6), box = 1 << box_log2, boxes_log2 = 6 - box_log2;
       const int held_log2 = 5 - boxes_log2, held = 1 << held_log2;
       int g = 0, queries = 0;  // blocks and query tiles copied so far
+      int index = blockIdx.x;   // of the piece; the ones after the first come from the queue
+      auto claim = [&] {
+        if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
+      };
       // the copies of one piece; false when a wait gave up
       auto copy = [&](const Item& it) {
         const int n = __shfl_sync(0xffffffffu, it.n, 0), head = __shfl_sync(0xffffffffu, it.head, 0);
-        if (n == 0) return true;
+        if (n == 0) {
+          if (v == 0) claim();
+          return true;
+        }
         const bool two = it.rows > a.lane_rows;
         const int* table = a.b.page_table + (int64_t)it.seq * a.b.ld_table;
         auto load_entries = [&](int first) {
@@ -400,6 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             copies += page[x] >= 0;
           }
           if (!over(empty_bar(s), phase(g) ^ 1u)) return false;
+          // the next piece is asked for when this one's last keys are: the ring's blocks cover the answer's way
+          if (v == 0 && j == n - 1) claim();
           if (elect_one()) {
             mbar_expect_tx(full, copies * box * D * 2);
 #pragma unroll
@@ -422,10 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       } else {
         Finder<kKB> finder(a, &g_paged_tc_status);
         if (blockIdx.x == 0 && lane == 0) *a.n_split = min(finder.splits, a.split_cap);
-        const int G = gridDim.x, c = blockIdx.x;
         for (int t = 0;; ++t) {
           if (!over(item_empty(t), (uint32_t)(((t >> 1) & 1) ^ 1))) break;
-          const int index = t * G + ((t & 1) ? G - 1 - c : c);
+          index = __shfl_sync(0xffffffffu, index, 0);
           bool more = index < finder.total;
           if (more) {
             Piece p;
@@ -692,6 +701,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const bool cut = it.slot >= 0;
       if (cut && (it.slot >= a.slot_cap || it.split >= a.split_cap)) {
         // cannot be: the pieces were chosen to fit
+      } else if (cut && i * a.lane_rows + 32 * quad >= it.rows) {
+        // no row of this warp's
       } else if (cut) {
         // row-interleaved 16-byte pieces, so that a warp's stores are contiguous
         float4* po =
@@ -791,63 +802,106 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-// Joins the cut tiles' pieces in piece order: a CTA takes 32 rows (one warp's of
-// the chunk kernel) and 32 of their outputs, a thread one row and four outputs,
-// as the chunk kernel stored them. So small, because a few tiles in many pieces
-// are the common case and the reads' latency is what the join costs: a chunk of
-// 64 tokens over 8192 rows (8 tiles in 18 pieces) took 48 us with 128 threads
-// for 32 whole rows, and takes 31. The rows go out through shared memory.
+// Joins the cut tiles' pieces. An item is 32 rows of a tile (one warp's of the
+// chunk kernel) and `wide` of their 16-byte columns, as the chunk kernel stored
+// them; the CTA's warps share an item's columns and, where these are fewer than
+// the warps, its pieces, whose parts then meet in shared memory in a fixed
+// order. What bounds it is latency: a few tiles in many pieces are the common
+// case, so the items are as narrow as leaves each CTA one (a chunk of 64 tokens
+// over 8192 rows, 8 tiles in 18 pieces, took 48 us with a CTA for 32 whole rows
+// and 26 so), all of a thread's loads go out at once, and so do the descriptions
+// of a CTA's items, most of which have no rows where sequences bring few.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_chunks_kernel(const __grid_constant__ Args a) {
-  constexpr int kParts = D / 32, kPitch = 32 * 2 + 8;
-  __shared__ __align__(16) uint8_t rows_s[32 * kPitch];
+__global__ void __launch_bounds__(256, 4) join_chunks_kernel(const __grid_constant__ Args a) {
+  constexpr int kCols = D / 4;
+  __shared__ float4 part_s[8][32];
+  __shared__ float2 ml_s[8][32];
+  __shared__ __align__(16) uint2 rows_s[32][9];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t items = (int64_t)min(*a.n_split, a.split_cap) * 8 * kParts;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int d0 = 32 * (int)(it % kParts), group = (int)(it / kParts % 8);
-    const Split sp = a.splits[it / (8 * kParts)];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.queue = 0;
+  const int n = min(*a.n_split, a.split_cap);
+  int wide_log2 = 3;
+  while (wide_log2 > 0 && n * 8 * (kCols >> wide_log2) * 2 <= (int)gridDim.x) --wide_log2;
+  const int wide = 1 << wide_log2, parts = kCols >> wide_log2, ways = 8 >> wide_log2;
+  const int way = warp >> wide_log2, items = n * 8 * parts;
+  const int64_t step = a.l.n_kv_heads;
+  for (int base = blockIdx.x; base < items; base += 32 * gridDim.x) {
+    // this lane's item of the CTA's next 32
+    const int mine = base + lane * (int)gridDim.x;
+    Split sp = {};
+    if (mine < items) sp = a.splits[mine % n];
+    const int my_group = mine / n / parts, my_r0 = 32 * (my_group & 3);
     // a chunk kernel that gave up may have left a description unwritten: nothing is taken on trust
-    if (sp.pieces < 1 || sp.pieces > a.slot_cap || sp.slot0 < 0 ||
-        sp.slot0 + (sp.pieces - 1) * (int64_t)a.l.n_kv_heads >= a.slot_cap || sp.rows < 1 || sp.rows > a.tile_rows ||
-        sp.token0 < 0 || sp.token0 + (int64_t)((sp.rows - 1) / a.group) >= a.b.T || sp.head0 < 0 ||
-        sp.head0 > (a.l.n_kv_heads - 1) * a.group)
-      continue;
-    const int i = group >> 2, r0 = 32 * (group & 3);                     // lane of the tile, first row there
-    if (r0 >= a.lane_rows || i * a.lane_rows + r0 >= sp.rows) continue;  // the same for the whole block
-    const int64_t step = a.l.n_kv_heads;
-    const float2* ml = a.part_ml + (int64_t)sp.slot0 * kRowsChunk + 32 * group + lane;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o) +
-                       (((int64_t)sp.slot0 * 8 + group) * (D / 4) + d0 / 4 + warp) * 32 + lane;
-    float top = -INFINITY;
-#pragma unroll 8
-    for (int s = 0; s < sp.pieces; ++s) top = fmaxf(top, ml[s * step * kRowsChunk].x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < sp.pieces; ++s) {
-      const float2 x = ml[s * step * kRowsChunk];
-      const float4 u = po[s * step * 8 * (D / 4) * 32];
-      const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
-      sum += f * x.y;
-      acc.x += f * u.x;
-      acc.y += f * u.y;
-      acc.z += f * u.z;
-      acc.w += f * u.w;
+    const bool sound = sp.pieces >= 1 && sp.pieces <= a.slot_cap && sp.slot0 >= 0 &&
+                       sp.slot0 + (sp.pieces - 1) * step < a.slot_cap && sp.rows >= 1 && sp.rows <= a.tile_rows &&
+                       sp.token0 >= 0 && sp.token0 + (int64_t)((sp.rows - 1) / a.group) < a.b.T && sp.head0 >= 0 &&
+                       sp.head0 <= (a.l.n_kv_heads - 1) * a.group;
+    unsigned todo = __ballot_sync(0xffffffffu, mine < items && sound && my_r0 < a.lane_rows &&
+                                                   (my_group >> 2) * a.lane_rows + my_r0 < sp.rows);
+    for (; todo; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1, at = (base + src * (int)gridDim.x) / n;
+      const int group = at / parts, part = at - group * parts;
+      const int slot0 = __shfl_sync(0xffffffffu, sp.slot0, src), pieces = __shfl_sync(0xffffffffu, sp.pieces, src);
+      const int col = (part << wide_log2) + (warp & (wide - 1));
+      const float2* ml = a.part_ml + (int64_t)slot0 * kRowsChunk + 32 * group + lane;
+      const float4* po =
+          reinterpret_cast<const float4*>(a.part_o) + (((int64_t)slot0 * 8 + group) * kCols + col) * 32 + lane;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      // (m2, l2, u): maximum, sum and outputs to be added
+      auto add = [&](float m2, float l2, const float4& u) {
+        const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+        const float f = ex2(m - ref), f2 = ex2(m2 - ref);
+        m = top;
+        l = l * f + l2 * f2;
+        o.x = o.x * f + u.x * f2;
+        o.y = o.y * f + u.y * f2;
+        o.z = o.z * f + u.z * f2;
+        o.w = o.w * f + u.w * f2;
+      };
+      constexpr int kAhead = 4;
+      for (int s0 = way; s0 < pieces; s0 += kAhead * ways) {
+        float2 x[kAhead];
+        float4 u[kAhead];
+#pragma unroll
+        for (int y = 0; y < kAhead; ++y) {
+          const int64_t s = (s0 + y * ways) * step;
+          if (s0 + y * ways < pieces) {
+            x[y] = __ldcg(ml + s * kRowsChunk);
+            u[y] = __ldcg(po + s * 8 * kCols * 32);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < kAhead; ++y)
+          if (s0 + y * ways < pieces) add(x[y].x, x[y].y, u[y]);
+      }
+      if (ways > 1) {
+        part_s[warp][lane] = o;
+        ml_s[warp][lane] = make_float2(m, l);
+        __syncthreads();
+        if (way == 0)
+          for (int w = warp + wide; w < 8; w += wide) add(ml_s[w][lane].x, ml_s[w][lane].y, part_s[w][lane]);
+      }
+      // out through shared memory: `wide` threads a row, 8 bytes each
+      if (way == 0) {
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        rows_s[lane][warp] = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+      }
+      __syncthreads();
+      const int token0 = __shfl_sync(0xffffffffu, sp.token0, src), rows = __shfl_sync(0xffffffffu, sp.rows, src),
+                head0 = __shfl_sync(0xffffffffu, sp.head0, src);
+      const int q = threadIdx.x >> wide_log2, c = threadIdx.x & (wide - 1);
+      const int r = 32 * (group & 3) + q, g = (group >> 2) * a.lane_rows + r;
+      if (q < 32 && r < a.lane_rows && g < rows) {
+        const int tok = g * a.group_magic >> 16;
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(token0 + tok) * a.ld_out +
+                                  (int64_t)(head0 + g - tok * a.group) * D + 4 * ((part << wide_log2) + c)) =
+            rows_s[q][c];
+      }
+      __syncthreads();
     }
-    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-    *reinterpret_cast<uint2*>(rows_s + lane * kPitch + warp * 8) =
-        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-    __syncthreads();
-    const int q = threadIdx.x >> 3, g = i * a.lane_rows + r0 + q;  // 8 threads a row, 8 bytes each
-    if (r0 + q < a.lane_rows && g < sp.rows) {
-      const int tok = g * a.group_magic >> 16;
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(sp.token0 + tok) * a.ld_out +
-                                (int64_t)(sp.head0 + g - tok * a.group) * D + d0 + 4 * (threadIdx.x & 7)) =
-          *reinterpret_cast<const uint2*>(rows_s + q * kPitch + (threadIdx.x & 7) * 8);
-    }
-    __syncthreads();
   }
 }
 
@@ -868,9 +922,9 @@ int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
   kernel<<<(unsigned)grid, kThreads, kControl + Cfg<D>::kTiles, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) {
-    const int64_t items = 8 * (D / 32) * (most_tiles < a.target ? most_tiles : a.target);
+    const int64_t items = 8 * (D / 4) * (most_tiles < a.target ? most_tiles : a.target);  // at most
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(items < 148 * 8 ? items : 148 * 8));
+    cfg.gridDim = dim3((unsigned)(items < 148 * 4 ? items : 148 * 4));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
