@@ -6,7 +6,11 @@
 // lanes of up to 128 rows (one TMEM lane a row; whole tokens, so 126 rows in
 // groups of 3), over a range of 64-key blocks. Both lanes use a key or value
 // block from shared memory once it is there, so L2 sees half the traffic of
-// 128-row tiles.
+// 128-row tiles. Where a piece has at most 32 rows (a decoding sequence in a
+// batch with a chunk), both lanes serve the same rows, each half of the blocks,
+// and lane 0 adds lane 1's outputs to its own: 24 single tokens over up to 8000
+// rows beside a chunk of 512 tokens over 3000 took 131 us with lane 1 idle and
+// take 107.
 //
 //   S = Q K^T  (fp32, TMEM)  ->  p = 2^(s c - m), c = scale log2 e  ->  O += P V
 //
@@ -67,6 +71,7 @@ using namespace tc;
 
 constexpr int kKB = 64;              // keys of a block
 constexpr int kThreads = 384;
+constexpr int kSharedRows = 32, kSharedBlocks = 8;  // at most, at least: a piece that both lanes serve
 constexpr float kLazy = 8.0f;        // log2 of the growth of a row's maximum that O tolerates
 
 template <int D>
@@ -93,6 +98,7 @@ struct Item {
   int seq, head, row_first, tokens; // sequence, KV head, first row of q, tokens of the tile
   int pos0, rows;                   // position of the first token; rows of the tile
   int slot, split, piece, pieces;
+  int shared;                       // both lanes serve the same rows, each half of the blocks (copied in turn)
 };
 
 // What the roles share, before the tiles in shared memory (which begin on a
@@ -102,6 +108,7 @@ struct Control {
   Item items[2];
   int abort, issued[2], queries;
   uint32_t tmem;
+  float2 ml[32];                    // lane 1's maxima and sums of a shared piece
 };
 constexpr int kControl = 1024;
 static_assert(sizeof(Control) <= kControl && kControl + Cfg<128>::kTiles <= 227 * 1024, "shared memory per CTA");
@@ -283,7 +290,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   auto o_full = [&](int i) { return bars + 8 * (kB + 18 + i); };
   auto o_empty = [&](int i) { return bars + 8 * (kB + 20 + i); };
   auto drain_bar = [&](int i) { return bars + 8 * (kB + 22 + i); };
-  static_assert(kB + 24 <= 56, "barriers");
+  // lane 1's part of a shared piece
+  const uint32_t part_full = bars + 8 * (kB + 24), part_empty = bars + 8 * (kB + 25);
+  static_assert(kB + 26 <= 56, "barriers");
 
   if (threadIdx.x == 32) {
     for (int s = 0; s < 2 * kDepth; ++s) {
@@ -292,6 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 2);
+    mbar_init(part_full, 1);
+    mbar_init(part_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(item_full(i), 1);
       mbar_init(item_empty(i), 11);  // every warp but the finding one
@@ -357,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
       };
       // the copies of one piece; false when a wait gave up
-      auto copy = [&](const Item& it) {
+      auto copy_as = [&](const Item& it, auto is_shared) {
+        constexpr bool shared = decltype(is_shared)::value;
         const int n = __shfl_sync(0xffffffffu, it.n, 0), head = __shfl_sync(0xffffffffu, it.head, 0);
         if (n == 0) {
           if (v == 0) claim();
@@ -365,10 +377,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
         const bool two = it.rows > a.lane_rows;
         const int* table = a.b.page_table + (int64_t)it.seq * a.b.ld_table;
+        // copy j's block: of a shared piece the two halves in turn
+        auto first_key = [&](int j) {
+          return it.keys.block(it.j0 + (!shared ? j : (j >> 1) + (j & 1 ? n - (n >> 1) : 0))) * kKB;
+        };
         auto load_entries = [&](int first) {
           const int j = first + (lane >> boxes_log2);
           if (j >= n) return -1;
-          const int kb = it.keys.block(it.j0 + j) * kKB + (lane & ((1 << boxes_log2) - 1)) * box;
+          const int kb = first_key(j) + (lane & ((1 << boxes_log2) - 1)) * box;
           if (!(kb < it.keys.hi && (kb + box > it.keys.lo || kb < it.keys.sink_end))) return -1;
           const int page = table[kb >> a.l.page_log2];
           if (page < 0 || page >= a.l.num_pages) {
@@ -399,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
           const int s = v * kDepth + g % kDepth;
           const uint32_t full = full_bar(s), dst = smem_u32(smem + C::kOffRing + s * C::kTile);
-          const int r0 = (it.keys.block(it.j0 + j) * kKB) & (a.l.page_size - 1);
+          const int r0 = first_key(j) & (a.l.page_size - 1);
           int page[4], copies = 0;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -424,6 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           }
         }
         return true;
+      };
+      auto copy = [&](const Item& it) {
+        return __shfl_sync(0xffffffffu, it.shared, 0) ? copy_as(it, std::true_type{}) : copy_as(it, std::false_type{});
       };
       Item it;
       if (v == 1) {
@@ -456,6 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               x.split = p.split;
               x.piece = p.piece;
               x.pieces = p.pieces;
+              x.shared = x.rows <= kSharedRows && x.n >= kSharedBlocks;
               ctl.items[t & 1] = x;
             }
           }
@@ -483,7 +503,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         const int n = __shfl_sync(0xffffffffu, it.n, 0);
         if (n == 0) continue;
         const bool two = __shfl_sync(0xffffffffu, it.rows, 0) > a.lane_rows;
-        if (i == 1 && !two) {
+        const bool shared = __shfl_sync(0xffffffffu, it.shared, 0) != 0;
+        if (i == 1 && !two && !shared) {
           // nothing for this lane: it only passes everything on (no phase may
           // go by unseen, the next wait could not tell it from its own)
           ok = over(q_full, (uint32_t)(queries++ & 1));
@@ -496,63 +517,91 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             }
           continue;
         }
-        auto k_there = [&](int j) { return over(full_bar((gc + j) % kDepth), phase(gc + j)); };
-        auto qk = [&](int j) {  // scores of block j, into the buffer of block g + j - 2; its keys are there
-          const int s = (gc + j) % kDepth, b = (g + j) & 1;
-          const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
-          if (g + j >= 2 && !over(pv_done(i, b), (uint32_t)(((g + j - 2) >> 1) & 1))) return false;
-          fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              mma_f16(tm + 64 * b, qs + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
-                      sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
-            mma_commit(s_full(i, b));
-            mma_commit(empty_bar(s));
-            if (j == n - 1) mma_commit(q_empty);
-          }
-          return true;
-        };
-        ok = over(q_full, (uint32_t)(queries & 1));
-        ++queries;
-        for (int j = 0; ok && j < min(n, 2); ++j) ok = k_there(j) && qk(j);
-        // the epilogue has read the last tile's outputs
-        if (ok && tiles > 0) ok = over(o_empty(i), (uint32_t)((tiles - 1) & 1));
-        for (int j = 0; ok && j < n; ++j) {
-          // what can be waited for before P is: this block's values, the keys of the next but one
-          const int s = kDepth + (gc + j) % kDepth, kb = it.keys.block(it.j0 + j) * kKB, b = (g + j) & 1;
-          if (!(ok = over(full_bar(s), phase(gc + j)))) break;
-          if (kb + kKB > it.keys.hi || (kb < it.keys.lo && kb + kKB > it.keys.sink_end)) {
-            // rows that no row of the tile sees (both lanes' warps write the same zeros)
-            uint8_t* v = smem + C::kOffRing + s * C::kTile;
-            for (int r = lane; r < kKB; r += 32) {
-              const int key = kb + r;
-              if (!(key < it.keys.hi && (key >= it.keys.lo || key < it.keys.sink_end)))
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                  *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) =
-                      make_uint4(0, 0, 0, 0);
+        // (compiled apart: with a shared piece's index arithmetic a step of the others took 2 % longer)
+        auto serve = [&](auto is_shared) {
+          constexpr bool shared = decltype(is_shared)::value;
+          // of a shared piece's copies every other one is this lane's; it passes the others on
+          constexpr int step = shared ? 2 : 1;
+          const int first = shared ? i : 0, own = (n - first + step - 1) / step;
+          const uint64_t qt = qs - (shared ? i * (C::kQTile >> 4) : 0);
+          const int j0 = it.j0 + (first ? n - own : 0);
+          auto block = [&](int j) { return gc + first + j * step; };
+          // waits for keys (v = 0) or values (kDepth) of this lane's block j; those before it that are not its own
+          auto there = [&](int j, int v) {
+            const int at = block(j);
+            if (shared && at > gc) {
+              if (!over(full_bar(v + (at - 1) % kDepth), phase(at - 1))) return false;
+              if (lane == 0) mbar_arrive(empty_bar(v + (at - 1) % kDepth));
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-          if (j + 2 < n && !(ok = k_there(j + 2))) break;
-          const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
-          if (!(ok = over(p_full(i, b), (uint32_t)(((g + j) >> 1) & 1)))) break;
-          fence_after();
-          if (elect_one()) {
+            return over(full_bar(v + at % kDepth), phase(at));
+          };
+          auto k_there = [&](int j) { return there(j, 0); };
+          auto qk = [&](int j) {  // scores of block j, into the buffer of block g + j - 2; its keys are there
+            const int s = block(j) % kDepth, b = (g + j) & 1;
+            const uint64_t sk = sw128_desc(ring + (uint32_t)s * C::kTile);
+            if (g + j >= 2 && !over(pv_done(i, b), (uint32_t)(((g + j - 2) >> 1) & 1))) return false;
+            fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kKB / 16; ++k)
-              mma_ts(tm + 256, tm + 64 * b + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
-            mma_commit(pv_done(i, b));
-            if (j == n - 1) mma_commit(o_full(i));
-            mma_commit(empty_bar(s));
+              for (int k = 0; k < D / 16; ++k)
+                mma_f16(tm + 64 * b, qt + (k >> 2) * (C::kQHalf >> 4) + 2 * (k & 3),
+                        sk + (k >> 2) * (C::kHalf >> 4) + 2 * (k & 3), id_qk, k != 0 ? 1u : 0u);
+              mma_commit(s_full(i, b));
+              mma_commit(empty_bar(s));
+              if (j == own - 1) mma_commit(q_empty);
+            }
+            return true;
+          };
+          bool ok = over(q_full, (uint32_t)(queries & 1));
+          ++queries;
+          for (int j = 0; ok && j < min(own, 2); ++j) ok = k_there(j) && qk(j);
+          // the epilogue has read the last tile's outputs
+          if (ok && tiles > 0) ok = over(o_empty(i), (uint32_t)((tiles - 1) & 1));
+          for (int j = 0; ok && j < own; ++j) {
+            // what can be waited for before P is: this block's values, the keys of the next but one
+            const int s = kDepth + block(j) % kDepth, b = (g + j) & 1;
+            const int kb = it.keys.block(j0 + j) * kKB;
+            if (!(ok = there(j, kDepth))) break;
+            if (kb + kKB > it.keys.hi || (kb < it.keys.lo && kb + kKB > it.keys.sink_end)) {
+              // rows that no row of the tile sees (both lanes' warps write the same zeros)
+              uint8_t* v = smem + C::kOffRing + s * C::kTile;
+              for (int r = lane; r < kKB; r += 32) {
+                const int key = kb + r;
+                if (!(key < it.keys.hi && (key >= it.keys.lo || key < it.keys.sink_end)))
+#pragma unroll
+                  for (int c = 0; c < D / 8; ++c)
+                    *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + r * 128 + ((c & 7) << 4)) =
+                        make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+            if (j + 2 < own && !(ok = k_there(j + 2))) break;
+            const uint64_t sv = sw128_desc_mn(ring + (uint32_t)s * C::kTile, C::kHalf);
+            if (!(ok = over(p_full(i, b), (uint32_t)(((g + j) >> 1) & 1)))) break;
+            fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < kKB / 16; ++k)
+                mma_ts(tm + 256, tm + 64 * b + 8 * k, sv + k * (16 * 128 >> 4), id_pv, (j | k) != 0 ? 1u : 0u);
+              mma_commit(pv_done(i, b));
+              if (j == own - 1) mma_commit(o_full(i));
+              mma_commit(empty_bar(s));
+            }
+            // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
+            if (j + 2 < own) ok = qk(j + 2);
           }
-          // the scores of block j + 2 go where P_j was; those of j + 1 keep the softmax busy meanwhile
-          if (j + 2 < n) ok = qk(j + 2);
-        }
+          if (shared && block(own - 1) < gc + n - 1)  // the last block is the other lane's
+            for (int v = 0; ok && v <= kDepth; v += kDepth) {
+              const int s = v + (gc + n - 1) % kDepth;
+              ok = over(full_bar(s), phase(gc + n - 1));
+              if (ok && lane == 0) mbar_arrive(empty_bar(s));
+            }
+          g += own;
+          return ok;
+        };
+        ok = shared ? serve(std::true_type{}) : serve(std::false_type{});
         gc += n;
-        g += n;
         ++tiles;
       }
       // every MMA issued is done before TMEM is released, whoever gave up
@@ -568,26 +617,34 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     // ------------------------------------------------ softmax and epilogue
     const int i = (warp - 4) >> 2, quad = warp & 3;  // TMEM lane quarter = warp & 3
     const int r = 32 * quad + lane;                  // row of the lane
-    const int row = r < a.lane_rows ? i * a.lane_rows + r : INT_MAX;  // row of the tile
     const uint32_t tl = (uint32_t)(32 * quad) << 16;
     const uint32_t to = tmem + tl + 256 + 128 * i;
     // a scale of 0 weighs all seen keys alike: scores 0, so that masked ones can stay infinite
     const bool flat = a.scale_log2 == 0.f;
     const float c = flat ? 1.0f : a.scale_log2;
-    const int my_token = row < INT_MAX ? row * a.group_magic >> 16 : 0;
-    int g = 0, tiles = 0;  // this lane's blocks and tiles so far
+    int g = 0, tiles = 0, parts = 0;  // this lane's blocks and tiles, the shared pieces so far
     Item it;
     bool ok = true;
     for (int t = 0; ok && take(t, it); ++t) {
-      if (i == 1 && it.rows <= a.lane_rows) continue;
-      const int n = it.n;
+      const bool shared = it.shared != 0;
+      if (i == 1 && it.rows <= a.lane_rows && !shared) continue;
+      const int half = it.n >> 1, n = !shared ? it.n : i == 0 ? it.n - half : half;
+      const int j0 = it.j0 + (shared && i == 1 ? it.n - half : 0);
+      const int lane_of_rows = shared ? 0 : i;
+      const int row = r < a.lane_rows ? lane_of_rows * a.lane_rows + r : INT_MAX;  // row of the tile
       const bool valid = row < it.rows;
-      const int pos = valid ? it.pos0 + my_token : -1;
-      const int pos_min = it.pos0 + i * (a.lane_rows / a.group);
-      const int pos_max = it.pos0 + min(it.tokens, (i + 1) * (a.lane_rows / a.group)) - 1;
+      const bool idle = lane_of_rows * a.lane_rows + 32 * quad >= it.rows;  // no row is this warp's
+      const int pos = valid ? it.pos0 + (row * a.group_magic >> 16) : -1;
+      const int pos_min = it.pos0 + lane_of_rows * (a.lane_rows / a.group);
+      const int pos_max = it.pos0 + min(it.tokens, (lane_of_rows + 1) * (a.lane_rows / a.group)) - 1;
       float m = -INFINITY, l = 0.f;  // m: the reference, in log2 units
-      for (int j = 0; j < n; ++j) {
-        const int kb = it.keys.block(it.j0 + j) * kKB, b = (g + j) & 1;
+      if (idle)  // (what its rows of P hold stays in its rows of O)
+        for (int j = 0; ok && j < n; ++j) {
+          ok = over(s_full(i, (g + j) & 1), (uint32_t)(((g + j) >> 1) & 1));
+          if (ok && lane == 0) mbar_arrive(p_full(i, (g + j) & 1));
+        }
+      for (int j = idle ? n : 0; j < n; ++j) {
+        const int kb = it.keys.block(j0 + j) * kKB, b = (g + j) & 1;
         const uint32_t ts = tmem + tl + 128 * i + 64 * b;
         ok = over(s_full(i, b), (uint32_t)(((g + j) >> 1) & 1));
         if (!ok) break;
@@ -699,10 +756,56 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       if (!ok) break;
       fence_after();
       const bool cut = it.slot >= 0;
-      if (cut && (it.slot >= a.slot_cap || it.split >= a.split_cap)) {
+      if (shared && !idle) {
+        // lane 1's outputs, maxima and sums reach lane 0 through lane 1's staging
+        float4* part = reinterpret_cast<float4*>(smem + C::kOffOut + 4 * C::kOut) + lane;
+        if (i == 0) {
+          ok = over(part_full, (uint32_t)(parts & 1));
+          if (!ok) break;
+        }
+        const float2 other = i == 0 ? ctl.ml[lane] : make_float2(m, l);
+        const float top = fmaxf(m, other.x), ref = top == -INFINITY ? 0.f : top;
+        const float f0 = ex2(m - ref), f1 = ex2(other.x - ref);
+#pragma unroll 1
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t w[32];
+          tmem_ld(to + 32 * x, w);
+          tmem_ld_wait(w);
+          if (i == 1) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              part[(8 * x + y) * 32] = make_float4(__uint_as_float(w[4 * y]), __uint_as_float(w[4 * y + 1]),
+                                                   __uint_as_float(w[4 * y + 2]), __uint_as_float(w[4 * y + 3]));
+          } else {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const float4 u = part[(8 * x + y) * 32];
+              w[4 * y] = __float_as_uint(__uint_as_float(w[4 * y]) * f0 + u.x * f1);
+              w[4 * y + 1] = __float_as_uint(__uint_as_float(w[4 * y + 1]) * f0 + u.y * f1);
+              w[4 * y + 2] = __float_as_uint(__uint_as_float(w[4 * y + 2]) * f0 + u.z * f1);
+              w[4 * y + 3] = __float_as_uint(__uint_as_float(w[4 * y + 3]) * f0 + u.w * f1);
+            }
+            tmem_st(to + 32 * x, w);
+          }
+        }
+        if (i == 1) {
+          ctl.ml[lane] = make_float2(m, l);
+        } else {
+          tmem_st_wait();
+          l = l * f0 + other.y * f1;
+          m = top;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(i == 1 ? part_full : part_empty);
+      }
+      // (every warp of lane 1: the staging is theirs too, and no phase of the barrier may go by unseen)
+      if (shared && i == 1) ok = over(part_empty, (uint32_t)(parts & 1));
+      if (shared) ++parts;
+      if (!ok) break;
+      if (idle || (shared && i == 1)) {
+        // nothing to write
+      } else if (cut && (it.slot >= a.slot_cap || it.split >= a.split_cap)) {
         // cannot be: the pieces were chosen to fit
-      } else if (cut && i * a.lane_rows + 32 * quad >= it.rows) {
-        // no row of this warp's
       } else if (cut) {
         // row-interleaved 16-byte pieces, so that a warp's stores are contiguous
         float4* po =

@@ -427,3 +427,27 @@ def test_attention_workspace_refusals(ie, cuda):
         run_attention(ie, cuda, s, workspace=cuda.zeros(n - 1, dtype=cuda.uint8, device="cuda"))
     with pytest.raises(ValueError, match="contiguous"):
         run_attention(ie, cuda, s, workspace=cuda.zeros(16, dtype=cuda.uint8, device="cuda")[:1].expand(n))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 2, 64), (16, 1, 128), (6, 2, 64)])
+@pytest.mark.parametrize("kv_lens", [
+    [448, 449, 512, 300, 513],       # from 8 blocks of 64 keys on a few rows' blocks are shared out
+    [576, 577, 9000, 300, 20000],    # odd numbers of blocks, and cut tiles
+])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (530, 70), (100, 3)])
+def test_attention_few_rows_beside_a_chunk(ie, cuda, dt, heads, kv_heads, dim, kv_lens, window, sinks):
+    """Sequences of one to a few tokens in a batch with a chunk."""
+    few = 32 // (heads // kv_heads)
+    s = ref.make_batch([1, 2, few, 150, few + 1], kv_lens, heads=heads, kv_heads=kv_heads, dim=dim, dt=dt, page=32,
+                       seed=31)
+    a = check_attention(ie, cuda, s, window=window, sinks=sinks)
+    assert bool((run_attention(ie, cuda, s, window=window, sinks=sinks) == a).all())
+
+
+def test_attention_many_single_tokens_beside_a_chunk(ie, cuda):
+    """More pieces that both lanes serve than CTAs, next to others."""
+    kv_lens = [600 + 37 * b for b in range(30)] + [900]
+    check_attention(ie, cuda, ref.make_batch([1] * 30 + [300], kv_lens, heads=32, kv_heads=8, page=64, seed=32))
+    kv_lens = [500 + 19 * b for b in range(60)] + [900, 2000]
+    check_attention(ie, cuda, ref.make_batch([1, 2] * 30 + [300, 60], kv_lens, heads=16, kv_heads=4, dim=64, seed=33))
