@@ -645,11 +645,12 @@ extern "C" int ie_paged_attention(ie_dtype dt, int B, int T, int max_q, int n_q_
     const int64_t by_rows = (int64_t)T * group / rows + B;
     return cache->n_kv_heads * (by_seq < by_rows ? by_seq : by_rows);
   };
-  // Up to 32 rows a sequence and head the few-rows kernel, in one or two tiles:
-  // at 20 and 32 rows it takes 72 us where the chunk kernel takes 85 (32
-  // sequences of 2048 rows) and 117 where that takes 130 (8 of 16384); at 64
-  // rows, in four tiles, 142 against 87.
-  const bool few = (int64_t)max_q * group <= 2 * kRowsFew;
+  // Up to 16 rows a sequence and head the few-rows kernel; 17 to 32, which it
+  // takes as two tiles, only for fewer than 32 sequences: with 20 rows it needs
+  // 12 us where the chunk kernel needs 16 (8 sequences of 300 cached rows) and 28
+  // where that needs 31 (8 of 2000), both need 61 (32 of 2048), and then it needs
+  // 76 against 69 (64 of 1000) and 369 against 351 (128 of 4000).
+  const bool few = (int64_t)max_q * group <= (B < 32 ? 2 * kRowsFew : kRowsFew);
   const int keys = few ? kKB : 64, box = a.l.page_size < keys ? a.l.page_size : keys;
   if (!make_map(&a.tmK, dt, cache->k, D, a.l, box, a.swap_rc) ||
       !make_map(&a.tmV, dt, cache->v, D, a.l, box, a.swap_rc))

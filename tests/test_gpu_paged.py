@@ -451,3 +451,10 @@ def test_attention_many_single_tokens_beside_a_chunk(ie, cuda):
     check_attention(ie, cuda, ref.make_batch([1] * 30 + [300], kv_lens, heads=32, kv_heads=8, page=64, seed=32))
     kv_lens = [500 + 19 * b for b in range(60)] + [900, 2000]
     check_attention(ie, cuda, ref.make_batch([1, 2] * 30 + [300, 60], kv_lens, heads=16, kv_heads=4, dim=64, seed=33))
+
+
+@pytest.mark.parametrize("B", [31, 32])
+def test_attention_verification_batches(ie, cuda, B):
+    """Five tokens a sequence, on both sides of the rule that picks the kernel."""
+    q_lens = [5 - b % 3 for b in range(B)]
+    check_attention(ie, cuda, ref.make_batch(q_lens, [5 + (b * 97) % 1300 for b in range(B)], seed=34))
