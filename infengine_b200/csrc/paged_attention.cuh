@@ -325,7 +325,7 @@ struct Finder {
     if (b < a.b.B) {
       s = sequence(a, b);
       tiles = tile_count(a, s);
-      most = most_blocks<KB>(a, s);
+      most = tiles ? most_blocks<KB>(a, s) : 0;
       if (s.bad && tell) atomicExch(status, IE_ERR_INVALID_ARG);
     }
   }
@@ -389,7 +389,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
       if (tid < a.b.B) {
         s = sequence(a, tid);
         tiles = tile_count(a, s);
-        most = most_blocks<KB>(a, s);
+        most = tiles ? most_blocks<KB>(a, s) : 0;
         if (s.bad && index == 0) atomicExch(status, IE_ERR_INVALID_ARG);
       }
       const int C = piece_blocks_by_waves(a, tiles * nkv, most);

@@ -458,3 +458,12 @@ def test_attention_verification_batches(ie, cuda, B):
     """Five tokens a sequence, on both sides of the rule that picks the kernel."""
     q_lens = [5 - b % 3 for b in range(B)]
     check_attention(ie, cuda, ref.make_batch(q_lens, [5 + (b * 97) % 1300 for b in range(B)], seed=34))
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([0, 1, 3], [9000, 40, 700]), ([0, 90, 1], [9000, 500, 700])])
+def test_attention_long_sequence_without_new_tokens(ie, cuda, q_lens, kv_lens):
+    """A slot that keeps its length but brings no rows does not change the others' bits."""
+    s = ref.make_batch(q_lens, kv_lens, seed=35)
+    a = check_attention(ie, cuda, s)
+    s["kv_len"][0] = 0
+    assert bool((run_attention(ie, cuda, s) == a).all())
