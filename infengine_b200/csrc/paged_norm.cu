@@ -54,8 +54,15 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   for (int i = 0; i < 8; ++i) e[i] = DT<T>::from_f(f[i]);
   return r;
 }
-// plain (coherent) load: q_out may alias q
-__device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+// coherent (q_out may alias q) and past L1, which no row visits twice: 53.2 -> 52.4 us at 11204 tokens
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p)
+               : "memory");
+  return r;
+}
 
 template <typename T, int D, int kHeads>
 __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const __grid_constant__ NormArgs a) {
