@@ -301,6 +301,13 @@ class TPStep:
 
 
 # ---------------------------------------------------------- reference arm
+REFERENCE_MISSING = "the reference's libraries (oracle/_ref) are not built: its source tree is absent"
+
+
+def reference_built():
+    return all((ROOT / "oracle" / "_ref" / n).exists() for n in ("libinfengine_ref.so", "libref_model_ref.so"))
+
+
 class RefStep:
     def __init__(self, torch, dev, seed):
         sys.path.insert(0, str(ROOT / "tests"))
@@ -1071,6 +1078,9 @@ def main():
         if rank != 0:  # the reference runs on one GPU; other ranks have no work
             return
         world = 1
+        if not reference_built():
+            emit({"impl": "reference", "unavailable": REFERENCE_MISSING})
+            return
     if world > 1:
         from datetime import timedelta
         torch.cuda.set_device(local)
@@ -1288,7 +1298,9 @@ def run_ours(torch, dist, dev, args, world, rank, local, hbm_peak, tf_peak, tf_p
         # BASELINE configs 1-4 one by one (before the long prefill chain, which
         # leaves the GPU warm and power-capped)
         result["configs"] = per_config(torch, step, stream, hbm_peak, tf_peak)
-        if not args.no_reference_configs:
+        if not reference_built():
+            result["configs_reference"] = {"unavailable": REFERENCE_MISSING}
+        elif not args.no_reference_configs:
             ref_cfg = reference_configs(torch, dev, args.seed)
             result["configs_reference"] = ref_cfg
             result["configs_speedup_vs_reference"] = versus_reference(result["configs"], ref_cfg)
@@ -1354,7 +1366,9 @@ def run_ours(torch, dist, dev, args, world, rank, local, hbm_peak, tf_peak, tf_p
         del eng5, es5
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
-        if args.parity_steps > 0:
+        if not reference_built():
+            result["parity"] = {"unavailable": REFERENCE_MISSING}
+        elif args.parity_steps > 0:
             result["parity"] = parity_leg(torch, dev, args.seed, args.parity_steps)
         if not args.no_cpu_baseline:
             result["cpu_baseline"] = cpu_baseline(args.seed)
