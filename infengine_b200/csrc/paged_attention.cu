@@ -6,8 +6,9 @@
 //
 // in one pass with a running maximum m (base 2, scale * log2 e folded into one
 // factor), fp32 throughout; p_j is rounded to the storage type for the tensor
-// cores and the sum takes the rounded values, so a rounding of p moves weight
-// between keys but not the total.
+// cores (fp16 with the maximum at 2^15, see paged_attention.cuh) and the sum
+// takes the rounded values, so a rounding of p moves weight between keys but not
+// the total.
 //
 // few_rows_kernel (at most 16 (token, head) rows a tile: decode, verification
 // of a few draft tokens). What bounds it: a cache row of 512 bytes costs
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  constexpr float kTop = DT<T>::id == IE_DTYPE_F16 ? kLargestLog2F16 : 0.f;  // log2 of the largest p
   const int pos_min = sq.pos0 + tok0, pos_max = sq.pos0 + tok1;
   auto wait = [&](int i) {
     const uint32_t bar = bar_u + 8 * (i % kSlots), parity = (uint32_t)((i / kSlots) & 1);
@@ -303,12 +305,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const __grid_cons
         m[x] = mx[x];
       }
     }
+    const float one[2] = {base[0] - kTop, base[1] - kTop};  // the score whose p is 1
     uint32_t pa[kKB / 16][4];
 #pragma unroll
     for (int i = 0; i < kKB / 8; ++i) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t w = pack2<T>(ex2(s[i][2 * x] - base[x]), ex2(s[i][2 * x + 1] - base[x]));
+        const uint32_t w = pack2<T>(ex2(s[i][2 * x] - one[x]), ex2(s[i][2 * x + 1] - one[x]));
         const float2 r = unpack2<T>(w);
         l[x] += r.x + r.y;
         pa[i >> 1][2 * (i & 1) + x] = w;

@@ -11,12 +11,22 @@
 // maxima and sums meet in the workspace and are joined in piece order (by the
 // tile's last CTA or by a second kernel). All of it is computed on the device from the lengths, so a
 // captured graph follows them.
+//
+// Probabilities p = 2^(x - m) meet the values in the storage type. fp16 has no
+// normal number below 2^-14 and none at all below 2^-25, so with the maximum at
+// 1 a long tail of small p vanished: 131070 keys 17.5 nats below one of value 0
+// gave 0 for 0.0033. Its range above 1 is free: both kernels hold p of fp16 as
+// p 2^k, k such that the largest is 2^15 (65504 is the type's), in the product
+// and in the sum, where it cancels; half a subnormal step is then 2^-32 of the
+// largest p or less. bf16 has the range of fp32 and needs none (k = 0).
 #pragma once
 #include <cuda.h>
 #include "paged.cuh"
 
 namespace ie {
 namespace pa {
+
+constexpr float kLargestLog2F16 = 15.0f;  // of a p in fp16
 
 struct Split {     // one tile that was cut, for the joining kernel
   int slot0, pieces, token0, rows, head0, row0, pad0, pad1;

@@ -15,10 +15,11 @@
 //   S = Q K^T  (fp32, TMEM)  ->  p = 2^(s c - m), c = scale log2 e  ->  O += P V
 //
 // The running maximum m is lazy: O is rescaled only when a row's maximum rises
-// by more than 2^8 over the reference it uses; p then stays below 2^8, which
-// neither type's rounding nor the fp32 sums notice, and after the first blocks
-// nearly no row needs it. p is rounded to the storage type for the product, the
-// sum takes the unrounded values.
+// by more than 2^8 over the reference it uses, and after the first blocks nearly
+// no row needs it. p then stays below 2^8, which bf16 and the fp32 sums do not
+// notice; of fp16 the reference's p is 2^7, so that the largest is 2^15 at most
+// and 2^7 at least (paged_attention.cuh says why). p is rounded to the storage
+// type for the product, the sum takes the unrounded values.
 //
 // What bounds it: 128 x 128 scores cost 1024 cycles of tensor work (D = 128)
 // and 1024 cycles of exponentials on the special-function unit (16 a cycle and
@@ -72,7 +73,12 @@ using namespace tc;
 constexpr int kKB = 64;              // keys of a block
 constexpr int kThreads = 384;
 constexpr int kSharedRows = 32, kSharedBlocks = 8;  // at most, at least: a piece that both lanes serve
-constexpr float kLazy = 8.0f;        // log2 of the growth of a row's maximum that O tolerates
+// log2 of the growth of a row's maximum that O tolerates (4 would keep 16 times
+// more of an fp16 tail; the rescaling it brings took a mixed batch of wide
+// scores from 152 to 165 us), and of the reference's p
+constexpr float kLazy = 8.0f;
+template <typename T>
+constexpr float kRefLog2 = DT<T>::id == IE_DTYPE_F16 ? kLargestLog2F16 - kLazy : 0.f;
 
 template <int D>
 struct Cfg {
@@ -718,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           l *= f;
           m = to_m;
         }
-        const float mb = m == -INFINITY ? 0.f : -m;
+        const float mb = kRefLog2<T> - (m == -INFINITY ? 0.f : m);
         const uint64_t c2 = pair(c, c), mb2 = pair(mb, mb);
         uint64_t l2 = pair(0.f, 0.f);
         uint32_t pk[kKB / 2];
