@@ -91,9 +91,10 @@ struct Cfg {
   static constexpr int kOffRing = 2 * kQTile;
   static constexpr int kOffOut = kOffRing + 2 * kDepth * kTile;
   static constexpr int kTiles = kOffOut + 8 * kOut;
-  // Of 8 pairs of exponentials, those on the FMA pipes (0, 2, 3, 4 and 8 took
-  // 1970, 1880, 1830, 1990 and 2590 cycles a step at D = 64).
-  static constexpr int kPoly = 3;
+  // Of 8 pairs of exponentials, those on the FMA pipes: 2 and 3 took 103.1 and
+  // 105.5 us over windows of 1024 (D = 64), 161.3 and 162.3 for a mixed batch
+  // (D = 128); 0, 2, 4 and 8 took 1970, 1880, 1990 and 2590 cycles a step at D = 64.
+  static constexpr int kPoly = 2;
 };
 
 // A piece of work, as the roles need it.
@@ -154,18 +155,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 // (2^a, 2^b) on the FMA pipes, for values up to 2^22: the nearest integer n by
 // adding 1.5 * 2^23, 2^f for the rest f in [-1/2, 1/2] by the polynomial of
-// degree 4 of least relative error (2^-18.5; degree 5, 2^-22.1, took 3 % longer
-// a step), n added to the exponent field. Values below -126 count as -126.
+// degree 5 of least relative error (2^-22.1 as evaluated: like ex2.approx's
+// 2^-22, so that a column's accuracy does not depend on which of the two it
+// gets; degree 4, 2^-18.5, was 0.6 % faster over windows), n added to the
+// exponent field. Values below -126 count as -126.
 __device__ __forceinline__ void ex2_poly2(float& a, float& b) {
   const uint64_t x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
   const float big = 12582912.0f;
   const uint64_t r = add2(x, pair(big, big));
   const uint64_t f = fma2(add2(r, pair(-big, -big)), pair(-1.0f, -1.0f), x);
   auto c = [](float v) { return pair(v, v); };
-  uint64_t p = fma2(c(9.570102e-3f), f, c(5.591786e-2f));
-  p = fma2(p, f, c(2.4024744e-1f));
-  p = fma2(p, f, c(6.931218e-1f));
-  p = fma2(p, f, c(9.999993e-1f));
+  uint64_t p = fma2(c(1.3276472e-3f), f, c(9.675541e-3f));
+  p = fma2(p, f, c(5.550713e-2f));
+  p = fma2(p, f, c(2.4022120e-1f));
+  p = fma2(p, f, c(6.9314694e-1f));
+  p = fma2(p, f, c(1.0000001f));
   float r0, r1, p0, p1;
   split(r, r0, r1);
   split(p, p0, p1);

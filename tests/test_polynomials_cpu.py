@@ -1,0 +1,28 @@
+"""CPU: the polynomials the kernels evaluate in place of 2^x, from the
+coefficients in their sources, against 2^x in higher precision."""
+import re
+from pathlib import Path
+
+import numpy as np
+
+CSRC = Path(__file__).resolve().parent.parent / "infengine_b200" / "csrc"
+NUMBER = r"([-+]?\d[\d.]*(?:e[-+]?\d+)?)"
+
+
+def body(source, function):
+    """The text of a function, from its name to the brace that ends its first line's column."""
+    text = (CSRC / source).read_text()
+    return re.search(r"\b" + function + r"\(.*?\n}\n", text, re.S).group(0)
+
+
+def test_chunk_attention_polynomial():
+    """No less exact than the hardware's ex2.approx (2^-22), so that a column's
+    accuracy does not depend on which of the two its place gives it. fp32
+    fused multiply-adds, as evaluated; one part in 16 for their roundings."""
+    c = [np.float32(x) for x in re.findall(r"c\(" + NUMBER + r"f\)", body("paged_attention_tc.cu", "ex2_poly2"))]
+    f = np.linspace(-0.5, 0.5, 400001).astype(np.float32)
+    p = np.full_like(f, c[0])
+    for x in c[1:]:  # (the product is exact in 64 bits)
+        p = (p.astype(np.float64) * f.astype(np.float64) + np.float64(x)).astype(np.float32)
+    off = np.abs(p.astype(np.float64) / np.exp2(f.astype(np.float64)) - 1).max()
+    assert off <= 2.0 ** -22 * 17 / 16, np.log2(off)
