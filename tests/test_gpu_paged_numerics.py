@@ -1,12 +1,28 @@
-"""GPU: paged attention where its arithmetic is strained."""
+"""GPU: paged attention where its arithmetic is strained: rows that one key
+takes, weight spread over a long tail of small probabilities, equal values."""
 import math
 
 import pytest
 
+import paged_bounds as pb
 import paged_ref as ref
 from test_gpu_paged import run_attention
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind,q_lens,kv_lens", pb.PEAKED)
+@pytest.mark.parametrize("q_factor,key_factor", [(1, 1), (8, 1), (40, 1), (40, 100)])
+def test_peaked_scores(ie, cuda, dt, dim, kind, q_lens, kv_lens, q_factor, key_factor):
+    s = pb.peaked_batch(q_lens, kv_lens, dt, q_factor, key_factor, dim=dim)
+    want, bound = pb.attention(s, sum_of_rounded=kind == "few")
+    assert bool(bound.isfinite().all())
+    got = run_attention(ie, cuda, s)[:s["start"][-1]].double().reshape(want.shape)
+    assert ie.device_status() == 0
+    off = (got - want).abs()
+    assert bool((off <= bound).all()), f"{float((off / bound).max())} of the bound"
 
 
 def tail_batch(cuda, B, n, kv, gap, heads, kv_heads, dt, dim=64, page=64):
