@@ -26,6 +26,7 @@
 // scans the 2048 groups, its first warp makes the cuts by searching the scanned
 // groups and then one group's 32 values, and the CTA whose slice holds the
 // token looks for it.
+#include <atomic>
 #include <cooperative_groups.h>
 #include "ie_common.cuh"
 
@@ -541,41 +542,62 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   }
 }
 
+// A launch of M rows on clusters of N CTAs.
+struct Launch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  Launch(int M, int N, cudaStream_t st) {
+    cfg.gridDim = dim3((unsigned)M * N);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = N;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+};
+
+// Clusters of N CTAs that run at once on the current device (asked once), 0 on
+// failure. A CTA takes an SM and a cluster lies in one GPC, so there are fewer
+// than SMs / N: 15 of 8 and 33 of 4 on a B200 of 148 SMs, where that would be
+// 18 and 37.
+template <typename T, int N>
+int at_once() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  static std::atomic<int> known[64];
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n) return n;
+  auto kernel = sample_kernel<T, N>;
+  const Launch l(1, N, nullptr);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &l.cfg) != cudaSuccess || n < 1)
+    return 0;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <typename T, int N>
 int launch(const SampleArgs& a, int M, cudaStream_t st) {
-  auto kernel = sample_kernel<T, N>;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return IE_ERR_LAUNCH;
-  static bool configured[64] = {};
-  if (!configured[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-      return IE_ERR_LAUNCH;
-    configured[dev] = true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)M * N);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = N;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? IE_OK : IE_ERR_LAUNCH;
+  if (!at_once<T, N>()) return IE_ERR_LAUNCH;
+  const Launch l(M, N, st);
+  return cudaLaunchKernelEx(&l.cfg, sample_kernel<T, N>, a) == cudaSuccess ? IE_OK : IE_ERR_LAUNCH;
 }
 
 template <typename T>
 int dispatch(const SampleArgs& a, int M, cudaStream_t st) {
-  // As many CTAs a row as keep the rows within one wave of the 148 SMs, at
-  // least as many as the 16-bit counters need.
+  // As many CTAs a row as let all rows run at once, at least as many as the
+  // 16-bit counters need. Both sides of the borders, of 128256 logits: 16 rows
+  // take 32.9 us with 8 CTAs each and 18.2 with 4, 15 take 19.7 with 8; 34 rows
+  // take 31.7 with 4 and 21.5 with 2, 32 take 18.9 with 4.
   auto fits = [&](int n) { return (int64_t)a.V / 8 / n + 1 <= (kMaxSlice - 14) / 8; };
   if (!fits(8)) return IE_ERR_UNSUPPORTED;
-  if (M * 8 <= 148 || !fits(4)) return launch<T, 8>(a, M, st);
-  if (M * 4 <= 148 || !fits(2)) return launch<T, 4>(a, M, st);
-  if (M * 2 <= 148 || !fits(1)) return launch<T, 2>(a, M, st);
+  if (!fits(4) || M <= at_once<T, 8>()) return launch<T, 8>(a, M, st);
+  if (!fits(2) || M <= at_once<T, 4>()) return launch<T, 4>(a, M, st);
+  if (!fits(1) || M <= at_once<T, 2>()) return launch<T, 2>(a, M, st);
   return launch<T, 1>(a, M, st);
 }
 
