@@ -262,8 +262,11 @@ __device__ __forceinline__ int piece_blocks_by_ends(const Args& a, int tiles_hea
 }
 
 // Finds pieces for one warp, in increasing order of their index: sequences are
-// taken 32 at a time, one a lane. The first 32 are read once; the pieces'
-// length comes from the whole batch (by waves for up to 32 sequences).
+// taken 32 at a time, one a lane. Up to 32 sequences are read once, come in
+// descending order of their most blocks, and the pieces' length is chosen by
+// where the pieces end; more are read twice, come in the batch's order, and a
+// piece has an even share of the batch's blocks (so that a long chunk that
+// stands last starts last).
 template <int KB>
 struct Finder {
   const Args& a;

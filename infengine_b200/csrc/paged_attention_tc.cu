@@ -35,11 +35,12 @@
 // Operands are 64-dimension halves of 128-byte rows, 128-byte swizzle: Q and K
 // K-major, V MN-major as it arrives.
 //
-// One CTA an SM takes pieces from a queue (the longest come first) until none
-// is left, and every role runs ahead of the next as far as its buffers allow: a
-// CTA for each piece spent 10 us of a 30 us piece on finding it, the first
-// copies and the epilogue; a fixed share of the pieces for each CTA left a
-// ragged batch of 10 to 800 tokens over up to 5000 rows at 297 us for 194.
+// One CTA an SM takes pieces from a queue (in batches of up to 32 sequences the
+// longest come first, see Finder) until none is left, and every role runs ahead
+// of the next as far as its buffers allow: a CTA for each piece spent 10 us of a
+// 30 us piece on finding it, the first copies and the epilogue; a fixed share of
+// the pieces for each CTA left a ragged batch of 10 to 800 tokens over up to
+// 5000 rows at 297 us for 194.
 //
 // Warp roles: 0 finds the pieces and copies queries and keys, 2 values (TMA
 // boxes of up to 64 rows of one page; the lanes hold the next table entries),

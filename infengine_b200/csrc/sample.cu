@@ -99,9 +99,11 @@ __device__ __forceinline__ void load_chunks(const uint4* p, int c, int step, int
                               : make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);
 }
 
-// 2^x for x <= 0 in 64 bits: the nearest integer and the polynomial of degree 10
-// of least relative error (2.1e-16) on [-1/2, 1/2]. About a third of the library
-// exponential's instructions, and the 64-bit pipe is what masses wait for.
+// 2^x for x <= 0 in 64 bits: the nearest integer and a polynomial of degree 10
+// for the rest, fitted for the least relative error on [-1/2, 1/2] (2.8e-16 with
+// the coefficients as stored, before the roundings of its evaluation). About a
+// third of the library exponential's instructions, and the 64-bit pipe is what
+// masses wait for.
 __device__ __forceinline__ double exp2_neg(double x) {
   if (!(x > -1000.0)) return 0.0;
   const double big = 6755399441055744.0;  // 1.5 * 2^52
