@@ -301,11 +301,14 @@ class TPStep:
 
 
 # ---------------------------------------------------------- reference arm
-REFERENCE_MISSING = "the reference's libraries (oracle/_ref) are not built: its source tree is absent"
-
-
-def reference_built():
-    return all((ROOT / "oracle" / "_ref" / n).exists() for n in ("libinfengine_ref.so", "libref_model_ref.so"))
+def reference_missing():
+    """Why the reference's legs cannot run, None where its libraries are built."""
+    if all((ROOT / "oracle" / "_ref" / n).exists() for n in ("libinfengine_ref.so", "libref_model_ref.so")):
+        return None
+    from __graft_entry__ import reference_tree
+    if reference_tree() is not None:
+        return "the reference's libraries (oracle/_ref) are not built although its source tree is there: make -C oracle"
+    return "the reference's libraries (oracle/_ref) are not built: its source tree is absent"
 
 
 class RefStep:
@@ -1078,8 +1081,8 @@ def main():
         if rank != 0:  # the reference runs on one GPU; other ranks have no work
             return
         world = 1
-        if not reference_built():
-            emit({"impl": "reference", "unavailable": REFERENCE_MISSING})
+        if (missing := reference_missing()):
+            emit({"impl": "reference", "unavailable": missing})
             return
     if world > 1:
         from datetime import timedelta
@@ -1298,8 +1301,8 @@ def run_ours(torch, dist, dev, args, world, rank, local, hbm_peak, tf_peak, tf_p
         # BASELINE configs 1-4 one by one (before the long prefill chain, which
         # leaves the GPU warm and power-capped)
         result["configs"] = per_config(torch, step, stream, hbm_peak, tf_peak)
-        if not reference_built():
-            result["configs_reference"] = {"unavailable": REFERENCE_MISSING}
+        if (missing := reference_missing()):
+            result["configs_reference"] = {"unavailable": missing}
         elif not args.no_reference_configs:
             ref_cfg = reference_configs(torch, dev, args.seed)
             result["configs_reference"] = ref_cfg
@@ -1366,8 +1369,8 @@ def run_ours(torch, dist, dev, args, world, rank, local, hbm_peak, tf_peak, tf_p
         del eng5, es5
         torch.cuda.synchronize()
         torch.cuda.empty_cache()
-        if not reference_built():
-            result["parity"] = {"unavailable": REFERENCE_MISSING}
+        if (missing := reference_missing()):
+            result["parity"] = {"unavailable": missing}
         elif args.parity_steps > 0:
             result["parity"] = parity_leg(torch, dev, args.seed, args.parity_steps)
         if not args.no_cpu_baseline:
