@@ -70,7 +70,10 @@ int ie_device_status(int clear);
  * ns = 0 restores the default of 2 s; at most 60 s (IE_ERR_INVALID_ARG
  * above). Applies to the current device, to kernels that start after the
  * call, and to graphs captured before it (the kernels read the limit when
- * they run). A kernel that gives up still waits, for up to 2 s, for the copies
+ * they run). A wait on a barrier is suspended by the hardware for as long as a
+ * copy takes, so that a shorter limit is not noticed; of ie_paged_attention,
+ * calls made (or captured) while the limit is below 1 ms look at their barriers
+ * without suspending. A kernel that gives up still waits, for up to 2 s, for the copies
  * and MMAs it issued itself before it exits. The reference has no
  * counterpart (its kernels do not wait on one another). */
 int ie_set_wait_limit_ns(unsigned long long ns);

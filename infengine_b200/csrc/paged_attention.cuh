@@ -53,6 +53,7 @@ struct Args {
   int join;       // chunks: the joining kernel's time, in blocks
   int min_blocks; // smallest piece
   int slot_cap, split_cap;
+  bool polled;    // the waits' limit is short: the kernels that look at their barriers without suspending
   int* arrived;   // few rows: pieces done of each cut tile, 0 between calls
   int* queue;     // chunks: pieces handed out behind the first of each CTA, 0 between calls
   int* n_split;   // chunks: number of cut tiles, and what the joining kernel needs of each

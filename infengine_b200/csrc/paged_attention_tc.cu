@@ -273,11 +273,14 @@ __device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, volatil
   return mbar_wait(bar, parity, abort_flag, &g_paged_tc_status, &g_paged_tc_wait_ns);
 }
 // (the bounded loop stays out of the roles' code, which is long enough to be felt in the instruction cache)
+template <bool kPolled>
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_try(bar, parity) || wait_long(bar, parity, abort_flag);
+  if constexpr (kPolled) return mbar_poll(bar, parity, abort_flag, &g_paged_tc_status, &g_paged_tc_wait_ns);
+  else return mbar_try(bar, parity) || wait_long(bar, parity, abort_flag);
 }
 
-template <typename T, int D>
+// kPolled: for wait limits that a suspended wait would outlast.
+template <typename T, int D, bool kPolled>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Args a) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -351,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   // buffer g & 1.
   auto phase = [&](int g) { return (uint32_t)((g / kDepth) & 1); };
   auto over = [&](uint32_t bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, wait(bar, parity, abort_flag)) != 0;
+    return __all_sync(0xffffffffu, wait<kPolled>(bar, parity, abort_flag)) != 0;
   };
   // piece t's description; the slot is free for the next but one once every warp has its copy
   auto take = [&](int t, Item& it) {
@@ -1019,9 +1022,10 @@ __global__ void __launch_bounds__(256, 4) join_chunks_kernel(const __grid_consta
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPolled = false>
 int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
-  auto kernel = chunk_kernel<T, D>;
+  if (!kPolled && a.polled) return launch<T, D, true>(a, most_tiles, st);
+  auto kernel = chunk_kernel<T, D, kPolled>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return IE_ERR_LAUNCH;
   static bool configured[64] = {};

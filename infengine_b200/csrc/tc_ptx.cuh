@@ -36,6 +36,17 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Without the suspension of mbar_try, which lasts until the phase is complete or
+// for a time that the hardware chooses and that copies do not outlast.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait on an mbarrier phase: false when it gave up after *wait_ns_p
 // (IE_ERR_TIMEOUT recorded in *status, abort raised) or when another role
 // already raised the abort flag.
@@ -53,6 +64,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       return false;
     }
   }
+}
+// The same for limits that mbar_try's suspension would outlast: looks again and
+// again, and gives up once *wait_ns_p has passed.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                          const unsigned long long* wait_ns_p) {
+  const unsigned long long wait_ns = *wait_ns_p;
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_test(bar, parity)) {
+    if (*abort_flag) return false;
+    if (globaltimer() - t0 >= wait_ns) {
+      atomicExch(status, IE_ERR_TIMEOUT);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  return true;
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
