@@ -62,6 +62,34 @@ struct Args {
   float* part_o;    // few rows: [slot][16][D]; chunks: [slot][8 warps][D / 4][32 rows][4]
 };
 
+constexpr int kSMs = 148;  // what the work is cut for; more or fewer serve it too
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT<T>::id == IE_DTYPE_BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // One sequence's extents after clamping to what the call was given.
 struct Seq {
   int start, tokens, kv, pos0;  // first row of q, rows served, cache rows, position of the first row
@@ -481,9 +509,9 @@ __device__ __forceinline__ bool find_piece(const Args& a, int index, Scan& sc, i
 int launch_chunks(ie_dtype dt, int D, Args& a, int64_t most_tiles, cudaStream_t st);
 
 constexpr int kRowsFew = 16;         // tile_rows of the few-rows kernel
-constexpr int kTargetFew = 148 * 4;  // its pieces
+constexpr int kTargetFew = kSMs * 4;  // its pieces
 constexpr int kRowsChunk = 256;      // tile_rows of the chunk kernel, at most
-constexpr int kTargetChunk = 148;
+constexpr int kTargetChunk = kSMs;
 
 }  // namespace pa
 }  // namespace ie

@@ -121,20 +121,6 @@ struct Control {
 constexpr int kControl = 1024;
 static_assert(sizeof(Control) <= kControl && kControl + Cfg<128>::kTiles <= 227 * 1024, "shared memory per CTA");
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (DT<T>::id == IE_DTYPE_BF16)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // ---- two fp32 values at a time
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -195,17 +181,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
-                                            int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
 }
 // D (TMEM) (+)= A (TMEM) . B (shared memory descriptor)
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
@@ -1042,7 +1017,7 @@ int launch(Args& a, int64_t most_tiles, cudaStream_t st) {
   if (e == cudaSuccess) {
     const int64_t items = 8 * (D / 4) * (most_tiles < a.target ? most_tiles : a.target);  // at most
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(items < 148 * 4 ? items : 148 * 4));
+    cfg.gridDim = dim3((unsigned)(items < kSMs * 4 ? items : kSMs * 4));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
