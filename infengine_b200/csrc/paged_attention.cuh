@@ -294,8 +294,9 @@ __device__ __forceinline__ int piece_blocks_by_ends(const Args& a, int tiles_hea
 // taken 32 at a time, one a lane. Up to 32 sequences are read once, come in
 // descending order of their most blocks, and the pieces' length is chosen by
 // where the pieces end; more are read twice, come in the batch's order, and a
-// piece has an even share of the batch's blocks (so that a long chunk that
-// stands last starts last).
+// piece has an even share of the batch's blocks (a chunk of 512 tokens over 3000
+// rows beside 63 single tokens takes 213 to 217 us wherever it stands; one over
+// 30000 rows 464 first and 483 last).
 template <int KB>
 struct Finder {
   const Args& a;
